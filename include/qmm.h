@@ -306,6 +306,115 @@ QMM_API int qmm_attention_decode_fused_dev(const float* qkv_dev, size_t batch, i
 /* *p_dev += value, stream-ordered (advances a captured step's position). */
 QMM_API int qmm_add_int_dev(int* p_dev, int value, void* stream);
 
+/* ---- Serving over a paged key/value cache (device pointers, stream-ordered). -----------
+ * A layer's cache is a pool of pages shared by all sequences; each sequence
+ * has its own length, its own pages (a block table) and any number of query
+ * heads. One decode step of a layer: qmm_paged_append_dev (the new token's q,
+ * k, v), qmm_paged_attention_dev, and, under a cache budget,
+ * qmm_paged_evict_dev; after the lm_head, qmm_process_logits_dev. The
+ * reference keeps one dense f32 cache per sequence and has none of the other
+ * steps. Lengths, positions, slots and tables are read from device memory, so
+ * a captured step can be replayed as they advance; values outside their range
+ * are never dereferenced (each entry says what they do). */
+
+/* Cache element types (GGML ids, gguf/main/src/api/types.rs:8-12). */
+#define QMM_KV_F32 0
+#define QMM_KV_F16 1
+#define QMM_KV_BF16 30
+
+/* A layer's pages. Row (page p, kv head h, slot s) is head_dim values at
+ * k_dev + p * page_stride + h * head_stride + s * slot_stride, in elements, the
+ * same in v_dev. k_dev, v_dev and the strides are multiples of 16 bytes.
+ * head_dim: a multiple of 64, at most 256; page_size: a power of two, 16 to
+ * 1024; n_heads of the calls: a multiple of n_kv_heads. Slots [i * page_size,
+ * (i + 1) * page_size) of sequence s are on page table_dev[s * table_stride + i],
+ * i < max_pages; its capacity is max_pages * page_size (at most 2^31 - 1). An
+ * entry outside [0, n_pages) names no page: its slots are neither written nor
+ * attended to. */
+typedef struct qmm_paged_kv {
+    void* k_dev;
+    void* v_dev;
+    int dtype;
+    int n_kv_heads;
+    int head_dim;
+    int page_size;
+    long long n_pages;
+    long long page_stride;
+    long long head_stride;
+    long long slot_stride;
+    const int* table_dev;
+    int n_seqs;
+    int max_pages;
+    long long table_stride;
+} qmm_paged_kv;
+
+/* For each of `tokens` fused q|k|v rows ((n_heads + 2 n_kv_heads) head_dim
+ * floats, rows ld_qkv floats apart): per-head RMSNorm of q and k (q_norm_dev and
+ * k_norm_dev both null: none), rotation by row positions_dev[i] of the cos/sin
+ * tables [ctx][head_dim / 2] (pairs half a head apart, or, interleaved != 0,
+ * neighbours), q to q_out_dev [tokens][n_heads][head_dim], k and v rounded to the
+ * cache's type into slot slots_dev[i] of sequence seqs_dev[i] (seqs_dev null:
+ * sequence i). The (sequence, slot) pairs are distinct. A position outside
+ * [0, ctx) gives a zero q row and stores nothing; a slot or sequence outside the
+ * table stores nothing (padding rows carry slot -1). Pointers 16-byte aligned,
+ * ld_qkv a multiple of 4. (attention.rs:505-540, rope.rs:7-130) */
+QMM_API int qmm_paged_append_dev(const qmm_paged_kv* kv, const float* qkv_dev, size_t ld_qkv, size_t tokens,
+                                 int n_heads, const float* q_norm_dev, const float* k_norm_dev, float offset,
+                                 float eps, const float* cos_dev, const float* sin_dev, int ctx, int interleaved,
+                                 const int* positions_dev, const int* slots_dev, const int* seqs_dev,
+                                 float* q_out_dev, void* stream);
+
+/* One new token per sequence: out_dev [n_seqs][n_heads][head_dim] = softmax(scale
+ * q . k) v over the sequence's slots [max(0, n - window), n), n = lengths_dev[s]
+ * clamped to [0, capacity], window 0: all. A sequence without slots gives
+ * zeros. q rows ld_q floats apart (a multiple of 4; 16-byte aligned pointers).
+ * weights_dev and weights_out_dev (both or neither; they may be equal), f32
+ * [n_seqs][n_kv_heads][capacity]: out = in, plus at each attended slot the sum
+ * over the kv head's query heads of the slot's softmax weight. Workspace: the
+ * library's, of the current device and `stream`; reserve
+ * qmm_paged_attention_workspace_size bytes before a stream capture.
+ * (attention.rs:545-600) */
+QMM_API size_t qmm_paged_attention_workspace_size(const qmm_paged_kv* kv, int n_heads, int with_weights);
+QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, size_t ld_q, int n_heads,
+                                    const int* lengths_dev, float scale, int window, const float* weights_dev,
+                                    float* weights_out_dev, float* out_dev, void* stream);
+
+/* Brings every sequence down to at most `budget` slots, per kv head. Of a
+ * sequence with n = lengths_dev[s] > budget slots those are kept whose position
+ * positions_dev [n_seqs][n_kv_heads][capacity] is at least next_positions_dev[s]
+ * - recent, then those with the largest weights_dev (same shape; NaN ranks as
+ * -infinity), ties and a surplus of recent slots by the lowest slot. Kept slots
+ * at or above `budget` move, in slot order, into the evicted ones below it (k and
+ * v in place); weights_out_dev and positions_out_dev (not the inputs) hold the
+ * moved arrays, 0 and -1 beyond the new length; lengths_out_dev [n_seqs] (not
+ * lengths_dev) the new lengths. Workspace as above. */
+QMM_API size_t qmm_paged_evict_workspace_size(const qmm_paged_kv* kv, int budget);
+QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, const float* weights_dev,
+                                const int* positions_dev, const int* next_positions_dev, int budget, int recent,
+                                int* lengths_out_dev, float* weights_out_dev, int* positions_out_dev, void* stream);
+
+/* Logits [rows][vocab] (rows ld floats apart) before sampling, to out_dev (rows
+ * ld_out apart; may be logits_dev). Row i's history is the first token_lengths_dev[i]
+ * (clamped to [0, max_tokens]) ids of tokens_dev + i * ld_tokens, the first
+ * prompt_lengths_dev[i] of them the prompt. A token in the history: x > 0 ? x /
+ * repetition[i] : x * repetition[i]; in the history after the prompt, count
+ * times: x - frequency[i] * count - presence[i]. Then x + the values of the
+ * token's entries among the row's n_bias (at most 1024) bias_ids_dev, in list
+ * order. Then -infinity where bit t % 32 of word t / 32 of grammar state
+ * mask_rows_dev[i] of mask_dev [n_masks][ceil(vocab / 32)] is clear (a state
+ * outside [0, n_masks): no mask; mask_rows_dev null: state i). Null tokens_dev,
+ * bias_ids_dev or mask_dev: that step is left out; null prompt_lengths_dev: no
+ * prompt; null penalties: 1, 0, 0. Ids outside [0, vocab) are ignored. */
+#define QMM_MAX_BIAS 1024
+QMM_API int qmm_process_logits_dev(const float* logits_dev, size_t ld, size_t rows, size_t vocab,
+                                   const int* tokens_dev, size_t ld_tokens, size_t max_tokens,
+                                   const int* token_lengths_dev, const int* prompt_lengths_dev,
+                                   const float* repetition_dev, const float* presence_dev,
+                                   const float* frequency_dev, const int* bias_ids_dev,
+                                   const float* bias_values_dev, size_t n_bias, const int* mask_dev,
+                                   size_t n_masks, const int* mask_rows_dev, float* out_dev, size_t ld_out,
+                                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

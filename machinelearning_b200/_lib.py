@@ -30,6 +30,11 @@ Q4_1 = 3
 Q8_0 = 8
 BLOCK_BYTES = {Q4_0: 18, Q4_1: 20, Q8_0: 34}
 
+# cache element types of a paged key/value cache (GGML ids)
+KV_F32 = 0
+KV_F16 = 1
+KV_BF16 = 30
+
 # qmm_act
 ACT_F32 = 0
 ACT_Q8_0 = 1
@@ -96,6 +101,14 @@ SIGNATURES = {
     "qmm_attention_decode_fused_dev": (_I, [_P, _SZ, _I, _I, _I, _P, _P, _F, _F, _P, _P, _P, _I, _P, _P, _F, _P, _P,
                                             _P]),
     "qmm_add_int_dev": (_I, [_P, _I, _P]),
+    # serving over a paged key/value cache
+    "qmm_paged_append_dev": (_I, [_P, _P, _SZ, _SZ, _I, _P, _P, _F, _F, _P, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "qmm_paged_attention_workspace_size": (_SZ, [_P, _I, _I]),
+    "qmm_paged_attention_dev": (_I, [_P, _P, _SZ, _I, _P, _F, _I, _P, _P, _P, _P]),
+    "qmm_paged_evict_workspace_size": (_SZ, [_P, _I]),
+    "qmm_paged_evict_dev": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "qmm_process_logits_dev": (_I, [_P, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _SZ, _P, _P,
+                                    _SZ, _P]),
     # include/qmm_tp.h
     "qmm_weight_create_row_shard": (_I, [_I, _SZ, _SZ, _P, _SZ, _I, _I, _I, _P]),
     "qmm_tp_available": (_I, []),
@@ -113,6 +126,15 @@ SIGNATURES = {
     "qmm_tp_all_reduce_f32": (_I, [_P, _P, _SZ, _P]),
 }
 TP_UNIQUE_ID_BYTES = 128
+MAX_BIAS = 1024  # QMM_MAX_BIAS
+
+
+class PagedKv(ctypes.Structure):
+    """qmm_paged_kv (include/qmm.h)."""
+    _fields_ = [("k_dev", _P), ("v_dev", _P), ("dtype", _I), ("n_kv_heads", _I), ("head_dim", _I), ("page_size", _I),
+                ("n_pages", ctypes.c_longlong), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("slot_stride", ctypes.c_longlong), ("table_dev", _P),
+                ("n_seqs", _I), ("max_pages", _I), ("table_stride", ctypes.c_longlong)]
 
 
 class QmmError(RuntimeError):

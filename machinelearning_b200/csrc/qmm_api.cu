@@ -18,6 +18,7 @@
 #include "../../include/qmm_tp.h"
 #include "qmm_common.cuh"
 #include "qmm_kernels.cuh"
+#include "qmm_paged.cuh"
 
 namespace qmm {
 static std::atomic<unsigned long long> g_launches{0};
@@ -1003,4 +1004,243 @@ QMM_API int qmm_add_int_dev(int* p_dev, int value, void* stream) {
     if (!p_dev) return fail(QMM_ERR_INVALID_INPUT, "null pointer");
     cudaError_t e = launch_add_int(p_dev, value, (cudaStream_t)stream);
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "add int");
+}
+
+// ---- serving over a paged key/value cache ------------------------------------------
+namespace {
+
+// Runs an entry point's body; what the C++ runtime throws on the host (an
+// allocation that fails) becomes a status.
+template <typename F>
+int guarded(F&& body) {
+    try {
+        return body();
+    } catch (...) {
+        return QMM_ERR_INVALID_DATA;
+    }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The kernels' view of a caller's cache description.
+int paged_view(const qmm_paged_kv* in, PagedKv* out) {
+    if (!in || !in->k_dev || !in->v_dev || !in->table_dev) return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+    const int size = kv_type_size(in->dtype);
+    if (!size) return fail(QMM_ERR_DTYPE_MISMATCH, "cache type is not f32, f16 or bf16");
+    if (in->head_dim <= 0 || in->head_dim % 64 || in->head_dim > 256)
+        return fail(QMM_ERR_SHAPE_MISMATCH, "head_dim is not a multiple of 64, at most 256");
+    if (in->n_kv_heads <= 0 || in->n_kv_heads > 65535 || in->n_seqs < 0 || in->n_seqs > 65535 || in->max_pages <= 0 ||
+        in->n_pages < 0 || in->n_pages > INT32_MAX)
+        return fail(QMM_ERR_SHAPE_MISMATCH, "kv heads, sequences or pages out of range");
+    int shift = 0;
+    while ((1 << shift) < in->page_size && shift < 10) ++shift;
+    if (in->page_size < kMinPage || (1 << shift) != in->page_size)
+        return fail(QMM_ERR_SHAPE_MISMATCH, "page size is not a power of two from 16 to 1024");
+    if (((long long)in->max_pages << shift) > INT32_MAX)
+        return fail(QMM_ERR_SHAPE_MISMATCH, "a sequence's capacity exceeds 2^31 - 1 slots");
+    const long long row = in->head_dim;
+    if (in->page_stride < row || in->head_stride < row || in->slot_stride < row || in->table_stride < 0)
+        return fail(QMM_ERR_SHAPE_MISMATCH, "a cache stride is shorter than a row");
+    if (!aligned16(in->k_dev) || !aligned16(in->v_dev) || in->page_stride * size % 16 || in->head_stride * size % 16 ||
+        in->slot_stride * size % 16)
+        return fail(QMM_ERR_INVALID_INPUT, "misaligned cache (pointers and strides: 16 B)");
+    out->k = in->k_dev;
+    out->v = in->v_dev;
+    out->dtype = in->dtype;
+    out->nkv = in->n_kv_heads;
+    out->hd = in->head_dim;
+    out->page_shift = shift;
+    out->n_pages = in->n_pages;
+    out->page_stride = in->page_stride;
+    out->head_stride = in->head_stride;
+    out->slot_stride = in->slot_stride;
+    out->table = in->table_dev;
+    out->n_seqs = in->n_seqs;
+    out->max_pages = in->max_pages;
+    out->table_stride = in->table_stride;
+    return QMM_OK;
+}
+
+int check_heads(int n_heads, const PagedKv& kv) {
+    if (n_heads <= 0 || n_heads % kv.nkv || n_heads > 65535)
+        return fail(QMM_ERR_SHAPE_MISMATCH, "query heads are not a multiple of the kv heads");
+    return QMM_OK;
+}
+
+int paged_workspace(size_t need, void* stream, void** ws) {
+    *ws = nullptr;
+    if (!need) return QMM_OK;
+    const int dev = current_device();
+    if (dev < 0) return fail(QMM_ERR_NO_DEVICE, "no CUDA device");
+    return get_workspace(dev, stream, need, ws);
+}
+
+}  // namespace
+
+QMM_API int qmm_paged_append_dev(const qmm_paged_kv* kv, const float* qkv_dev, size_t ld_qkv, size_t tokens,
+                                 int n_heads, const float* q_norm_dev, const float* k_norm_dev, float offset,
+                                 float eps, const float* cos_dev, const float* sin_dev, int ctx, int interleaved,
+                                 const int* positions_dev, const int* slots_dev, const int* seqs_dev,
+                                 float* q_out_dev, void* stream) {
+    return guarded([&]() -> int {
+        AppendArgs a = {};
+        int rc = paged_view(kv, &a.kv);
+        if (!rc) rc = check_heads(n_heads, a.kv);
+        if (rc) return rc;
+        if (tokens == 0) return QMM_OK;
+        if (!qkv_dev || !cos_dev || !sin_dev || !positions_dev || !slots_dev || !q_out_dev ||
+            (q_norm_dev == nullptr) != (k_norm_dev == nullptr))
+            return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+        const size_t row = ((size_t)n_heads + 2 * (size_t)a.kv.nkv) * a.kv.hd;
+        // one grid row holds every head vector, at least eight to a CTA
+        if (ld_qkv < row || ctx <= 0 || tokens > (size_t)INT32_MAX ||
+            tokens * (row / a.kv.hd) > (size_t)INT32_MAX * 8)
+            return fail(QMM_ERR_SHAPE_MISMATCH, "row stride, context or token count out of range");
+        if (!aligned16(qkv_dev) || ld_qkv % 4 || !aligned16(cos_dev) || !aligned16(sin_dev) || !aligned16(q_out_dev) ||
+            !aligned16(q_norm_dev) || !aligned16(k_norm_dev))
+            return fail(QMM_ERR_INVALID_INPUT, "misaligned pointer (16 B) or row stride (4 floats)");
+        a.qkv = qkv_dev;
+        a.ld = (int64_t)ld_qkv;
+        a.tokens = (int)tokens;
+        a.nq = n_heads;
+        a.q_norm = q_norm_dev;
+        a.k_norm = k_norm_dev;
+        a.offset = offset;
+        a.eps = eps;
+        a.cos_t = cos_dev;
+        a.sin_t = sin_dev;
+        a.ctx = ctx;
+        a.positions = positions_dev;
+        a.slots = slots_dev;
+        a.seqs = seqs_dev;
+        a.q_out = q_out_dev;
+        const cudaError_t e = launch_paged_append(a, interleaved != 0, (cudaStream_t)stream);
+        return e == cudaSuccess ? QMM_OK : cuda_fail(e, "paged append");
+    });
+}
+
+QMM_API size_t qmm_paged_attention_workspace_size(const qmm_paged_kv* kv, int n_heads, int with_weights) {
+    PagedKv v;
+    if (guarded([&]() -> int {
+            const int rc = paged_view(kv, &v);
+            return rc ? rc : check_heads(n_heads, v);
+        }))
+        return 0;
+    return paged_attention_workspace(v, n_heads, with_weights != 0);
+}
+
+QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, size_t ld_q, int n_heads,
+                                    const int* lengths_dev, float scale, int window, const float* weights_dev,
+                                    float* weights_out_dev, float* out_dev, void* stream) {
+    return guarded([&]() -> int {
+        AttendArgs a = {};
+        int rc = paged_view(kv, &a.kv);
+        if (!rc) rc = check_heads(n_heads, a.kv);
+        if (rc) return rc;
+        if (a.kv.n_seqs == 0) return QMM_OK;
+        if (!q_dev || !lengths_dev || !out_dev || (weights_dev == nullptr) != (weights_out_dev == nullptr))
+            return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+        if (ld_q < (size_t)n_heads * a.kv.hd || window < 0)
+            return fail(QMM_ERR_SHAPE_MISMATCH, "query row stride or window out of range");
+        if (!aligned16(q_dev) || ld_q % 4 || !aligned16(out_dev))
+            return fail(QMM_ERR_INVALID_INPUT, "misaligned pointer (16 B) or row stride (4 floats)");
+        a.q = q_dev;
+        a.ldq = (int64_t)ld_q;
+        a.nq = n_heads;
+        a.lengths = lengths_dev;
+        a.scale = scale;
+        a.window = window;
+        a.weights = weights_dev;
+        a.weights_out = weights_out_dev;
+        a.out = out_dev;
+        void* ws = nullptr;
+        rc = paged_workspace(paged_attention_workspace(a.kv, n_heads, weights_dev != nullptr), stream, &ws);
+        if (rc) return rc;
+        const cudaError_t e = launch_paged_attention(a, ws, (cudaStream_t)stream);
+        return e == cudaSuccess ? QMM_OK : cuda_fail(e, "paged attention");
+    });
+}
+
+QMM_API size_t qmm_paged_evict_workspace_size(const qmm_paged_kv* kv, int budget) {
+    PagedKv v;
+    if (budget < 1 || guarded([&]() -> int { return paged_view(kv, &v); })) return 0;
+    return paged_evict_workspace(v, budget);
+}
+
+QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, const float* weights_dev,
+                                const int* positions_dev, const int* next_positions_dev, int budget, int recent,
+                                int* lengths_out_dev, float* weights_out_dev, int* positions_out_dev, void* stream) {
+    return guarded([&]() -> int {
+        EvictArgs a = {};
+        int rc = paged_view(kv, &a.kv);
+        if (rc) return rc;
+        if (a.kv.n_seqs == 0) return QMM_OK;
+        if (!lengths_dev || !weights_dev || !positions_dev || !next_positions_dev || !lengths_out_dev ||
+            !weights_out_dev || !positions_out_dev)
+            return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+        if (weights_out_dev == weights_dev || positions_out_dev == positions_dev || lengths_out_dev == lengths_dev)
+            return fail(QMM_ERR_INVALID_INPUT, "eviction does not write its inputs: pass separate outputs");
+        if (budget < 1 || recent < 0 || recent > budget)
+            return fail(QMM_ERR_SHAPE_MISMATCH, "budget below 1, or recent outside [0, budget]");
+        a.lengths = lengths_dev;
+        a.weights = weights_dev;
+        a.positions = positions_dev;
+        a.next_positions = next_positions_dev;
+        a.budget = budget;
+        a.recent = recent;
+        a.lengths_out = lengths_out_dev;
+        a.weights_out = weights_out_dev;
+        a.positions_out = positions_out_dev;
+        void* ws = nullptr;
+        rc = paged_workspace(paged_evict_workspace(a.kv, budget), stream, &ws);
+        if (rc) return rc;
+        const cudaError_t e = launch_paged_evict(a, ws, (cudaStream_t)stream);
+        return e == cudaSuccess ? QMM_OK : cuda_fail(e, "paged evict");
+    });
+}
+
+QMM_API int qmm_process_logits_dev(const float* logits_dev, size_t ld, size_t rows, size_t vocab,
+                                   const int* tokens_dev, size_t ld_tokens, size_t max_tokens,
+                                   const int* token_lengths_dev, const int* prompt_lengths_dev,
+                                   const float* repetition_dev, const float* presence_dev,
+                                   const float* frequency_dev, const int* bias_ids_dev,
+                                   const float* bias_values_dev, size_t n_bias, const int* mask_dev,
+                                   size_t n_masks, const int* mask_rows_dev, float* out_dev, size_t ld_out,
+                                   void* stream) {
+    return guarded([&]() -> int {
+        if (rows == 0 || vocab == 0) return QMM_OK;
+        if (!logits_dev || !out_dev || (tokens_dev && !token_lengths_dev) || (bias_ids_dev && !bias_values_dev))
+            return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+        if (rows > 65535 || vocab > (size_t)INT32_MAX - 65536 || ld < vocab || ld_out < vocab || n_bias > kMaxBias ||
+            n_masks > (size_t)INT32_MAX || max_tokens > (size_t)INT32_MAX || (tokens_dev && ld_tokens < max_tokens))
+            return fail(QMM_ERR_SHAPE_MISMATCH,
+                        "rows (at most 65535), vocabulary, row stride, history, biases (at most 1024) out of range");
+        if (mask_dev && !mask_rows_dev && n_masks < rows)
+            return fail(QMM_ERR_SHAPE_MISMATCH, "fewer masks than rows");
+        if (logits_dev == out_dev && ld != ld_out)
+            return fail(QMM_ERR_INVALID_INPUT, "in place, the row strides have to be equal");
+        LogitsArgs a = {};
+        a.logits = logits_dev;
+        a.ld = (int64_t)ld;
+        a.rows = (int)rows;
+        a.vocab = (int)vocab;
+        a.tokens = tokens_dev;
+        a.ld_tokens = (int64_t)ld_tokens;
+        a.max_tokens = (int)max_tokens;
+        a.token_lengths = token_lengths_dev;
+        a.prompt_lengths = prompt_lengths_dev;
+        a.repetition = repetition_dev;
+        a.presence = presence_dev;
+        a.frequency = frequency_dev;
+        a.bias_ids = bias_ids_dev;
+        a.bias_values = bias_values_dev;
+        a.n_bias = bias_ids_dev ? (int)n_bias : 0;
+        a.mask = mask_dev;
+        a.n_masks = (int)n_masks;
+        a.mask_rows = mask_rows_dev;
+        a.out = out_dev;
+        a.ld_out = (int64_t)ld_out;
+        const cudaError_t e = launch_process_logits(a, (cudaStream_t)stream);
+        return e == cudaSuccess ? QMM_OK : cuda_fail(e, "process logits");
+    });
 }
