@@ -328,7 +328,7 @@ QMM_API int qmm_add_int_dev(int* p_dev, int value, void* stream);
  * head_dim: a multiple of 64, at most 256; page_size: a power of two, 16 to
  * 1024; n_heads of the calls: a multiple of n_kv_heads. Slots [i * page_size,
  * (i + 1) * page_size) of sequence s are on page table_dev[s * table_stride + i],
- * i < max_pages; its capacity is max_pages * page_size (at most 2^31 - 1). An
+ * i < max_pages; its capacity is max_pages * page_size (at most 2^30). An
  * entry outside [0, n_pages) names no page: its slots are neither written nor
  * attended to. */
 typedef struct qmm_paged_kv {

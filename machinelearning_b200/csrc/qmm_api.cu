@@ -1036,8 +1036,8 @@ int paged_view(const qmm_paged_kv* in, PagedKv* out) {
     while ((1 << shift) < in->page_size && shift < 10) ++shift;
     if (in->page_size < kMinPage || (1 << shift) != in->page_size)
         return fail(QMM_ERR_SHAPE_MISMATCH, "page size is not a power of two from 16 to 1024");
-    if (((long long)in->max_pages << shift) > INT32_MAX)
-        return fail(QMM_ERR_SHAPE_MISMATCH, "a sequence's capacity exceeds 2^31 - 1 slots");
+    if (((long long)in->max_pages << shift) > (1 << 30))
+        return fail(QMM_ERR_SHAPE_MISMATCH, "a sequence's capacity exceeds 2^30 slots");
     const long long row = in->head_dim;
     if (in->page_stride < row || in->head_stride < row || in->slot_stride < row || in->table_stride < 0)
         return fail(QMM_ERR_SHAPE_MISMATCH, "a cache stride is shorter than a row");

@@ -7,6 +7,17 @@
 // slots; m is the largest score. A sequence without slots gives zeros.
 // Optionally every slot's weight sum over the kv head's query heads of
 // e^(s_t - m) / sum e^(s - m) is added to a running total.
+//
+// What bounds it: every K and V element is read once and takes 2 g
+// multiply-adds (g query heads per kv head), so HBM, as long as the products
+// run on the tensor cores: at g = 8 in f32 on the CUDA cores they would take
+// most of the machine.
+//
+// One pass with a running maximum and sum (attend_kernel), the work divided
+// evenly over a fixed grid whatever the lengths are, then a join of the pieces
+// of sequences that were divided (join_kernel).
+#include <cuda_bf16.h>
+
 #include "qmm_common.cuh"
 #include "qmm_kernels.cuh"
 #include "qmm_paged.cuh"
@@ -15,145 +26,763 @@ namespace qmm {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kMaxHd = 256;
+constexpr int kHeadTile = 8;  // query heads of one kv head that share a pass over its K and V
+constexpr float kLog2e = 1.4426950408889634f;
 
+// ---- matrix instructions ----------------------------------------------------------
+// D (16 x 8, f32) += A (16 x 16, row) B (16 x 8, col); for f32 caches
+// D += A (16 x 8, tf32) B (8 x 8, tf32).
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 4)
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else if constexpr (std::is_same_v<T, __half>)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t tf32_rna(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+
+// x as hi + lo of the instruction's operand type: f32 arithmetic on 16-bit or
+// tf32 operands. What is left over is below 2^-16 |x| (bf16), 2^-22 |x|
+// (f16, tf32).
+template <typename T>
+__device__ __forceinline__ void split(float x, T* hi, T* lo) {
+    if constexpr (sizeof(T) == 4) {
+        *hi = __uint_as_float(tf32_rna(x));
+        *lo = __uint_as_float(tf32_rna(x - *hi));
+    } else {
+        *hi = f32_to_kv<T>(x);
+        *lo = f32_to_kv<T>(x - kv_to_f32<T>(*hi));
+    }
+}
+// The same for two values at once, packed (16-bit types).
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 f = __half22float2(h);
+        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+        *hi = *reinterpret_cast<const uint32_t*>(&h);
+        *lo = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        const float2 f = __bfloat1622float2(h);
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
+        *hi = *reinterpret_cast<const uint32_t*>(&h);
+        *lo = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22; 0 below 2^-126
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 16 bytes to shared memory, zeros where !live (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+__device__ __forceinline__ float quad_max(float v) {  // over the four lanes of a head
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// e^(m - M) of a piece's maximum m, 0 for a piece that saw no slot.
+__device__ __forceinline__ float piece_factor(float m, float M) { return m == -INFINITY ? 0.0f : exp2f(m - M); }
 
-__device__ __forceinline__ void slot_range(const AttendArgs& a, int b, int64_t* first, int64_t* n) {
+// ---- division of the work -----------------------------------------------------------
+// The slots [first, n) of a sequence, in steps ("tiles") of kSlots aligned slots.
+struct Slots {
+    int first, n;
+    int tile0, tiles;
+};
+template <int kSlots>
+__device__ __forceinline__ Slots slots_of(const AttendArgs& a, int b) {
+    Slots s;
     const int64_t cap = a.kv.capacity();
-    int64_t len = a.lengths[b];
-    len = len < 0 ? 0 : (len > cap ? cap : len);
-    *n = len;
-    *first = a.window > 0 && len > a.window ? len - a.window : 0;
+    const int len = a.lengths[b];
+    s.n = len < 0 ? 0 : (len > cap ? (int)cap : len);
+    s.first = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
+    s.tile0 = s.first / kSlots;
+    s.tiles = (s.n + kSlots - 1) / kSlots - s.tile0;
+    return s;
 }
 
-// One CTA per (query head, sequence): each warp takes every eighth slot with a
-// running maximum and sum, the warps are joined at the end.
+// A piece of the work: consecutive tiles of one (sequence, head tile). The
+// list of all (sequence, head tile)s, each kSetup units of starting and ending it
+// followed by one unit per tile, is cut into equal shares, one per CTA (without
+// the setup's units a CTA got dozens of short sequences where another had part
+// of one: 64 sequences of 1 to 8192 slots, 64/8 heads of 128, f16 took 238 us
+// instead of 101). Pieces that are not a whole (sequence, head tile) leave (acc, m, l)
+// behind: in the CTA's slot 0 if earlier CTAs hold the beginning, in slot 1 if not.
+struct Plan {
+    int first_cta, pieces;  // of a (sequence, head tile)
+};
+
+struct Scratch {
+    Plan* plans;     // [n_seqs][head tiles]
+    float2* ml;      // [grid][2][kHeadTile]: maximum (in units of log 2) and sum of a piece
+    float* acc;      // [grid][2][kHeadTile][hd]
+    float2* stats;   // [n_seqs][nq], with weights: the final maximum and sum
+    float* scores;   // [n_seqs][nq][capacity], with weights: scores in units of log 2
+    int head_tiles;  // per kv head
+};
+
+// kTile slots are the K of one instruction's P; a step takes kTiles of them. A
+// warp's ring holds three units of a step's K or V rows: one in use, two on
+// their way (16 warps per SM with 4 KB units: 128 KB in flight, above the 44 KB
+// that 6.5 TB/s and 1 us need).
+template <typename T, int HD>
+struct Shape {
+    static constexpr int kTile = sizeof(T) == 4 ? 8 : 16;
+    static constexpr int kTiles = HD <= 64 ? 2 : 1;
+    static constexpr int kSlots = kTile * kTiles;
+    static constexpr int kRow = HD * (int)sizeof(T);             // bytes
+    static constexpr int kChunks = kRow / 64;                    // 16-byte units of a K row per lane
+    static constexpr int kLines = kRow / 128;                    // of a row; 16-byte units of a V row per lane
+    static constexpr int kVRows = kTile / 4;                     // V rows of a tile per lane
+    static constexpr int kUnit = kSlots * HD * (int)sizeof(T);
+    static constexpr int kUnits = 3;
+    static constexpr int kWarps = HD <= 128 ? 8 : (HD <= 192 ? 5 : 4);
+    static constexpr int kCtas = 2;                              // per SM
+    static constexpr int kSetup = 65536 / (2 * kUnit);           // a piece's fixed cost in steps: about 3 us
+    static constexpr int kQBytes = kChunks * 2 * 32 * 16;
+    static constexpr bool kQRegs = kChunks <= (kWarps == 8 ? 4 : 8);  // Q in registers
+    static constexpr int kAccRow = HD + 4;                       // floats; spreads the rows over the banks
+    static constexpr size_t kSmem = (size_t)kWarps * kUnits * kUnit + kQBytes + kWarps * kHeadTile * 8 + kHeadTile * 4;
+    static_assert(kHeadTile * kAccRow * 4 <= kUnits * kUnit, "a warp's result fits in its ring");
+};
+
+// Weights are relative to 2^m with m at most kSlack below the largest score so
+// far (in units of log 2): the sums are rescaled when it grows by more, not at
+// every new maximum (a few times a warp). f16 holds 2^-24 to 2^16: there the
+// weights are scaled by 2^14, so that small ones keep their bits, and kSlack is 1.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a, float* scores, float2* stats) {
-    __shared__ float acc_s[kWarps][kMaxHd];
-    __shared__ float m_s[kWarps], l_s[kWarps];
-    const int h = blockIdx.x, b = blockIdx.y;
-    const int hd = a.kv.hd, per = hd / 32;
-    const int kvh = h / (a.nq / a.kv.nkv);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int64_t first, n;
-    slot_range(a, b, &first, &n);
-    const float* q = a.q + b * a.ldq + (int64_t)h * hd;
-    float qr[8], acc[8];
+constexpr float kWeightBias = std::is_same_v<T, __half> ? 14.0f : 0.0f;
+template <typename T>
+constexpr float kSlack = std::is_same_v<T, __half> ? 1.0f : 8.0f;
+
+// Every warp takes each kWarps-th step of the piece, and runs on its own until
+// the piece ends. The lane layout of the matrix instructions is met without a
+// transpose: lane (g, t) = (lane / 4, lane % 4)
+//  * as operand B of S = Q K^T holds K row g of 8 slots, at column pairs that
+//    depend on t. Which columns is free as long as Q has the same order, so it
+//    takes whole 16-byte units t, t + 4, ... of the row;
+//  * as operand A of O^T = V^T P^T holds rows (columns of V) g and g + 8, at the
+//    slot pairs 2 t, 2 t + 1 (+ 8, + 9). Which columns is free again: it takes 8
+//    (f32: 4) consecutive ones, two by two, and pairs two slots' values by byte
+//    permutes (16 bit).
+// S's layout is that of the operand B of V^T P^T: P stays in registers.
+// In S, operand A has 16 rows for the 8 heads of the tile: rows 0-7 are the high,
+// rows 8-15 the low parts of Q, so the products are those of f32 queries with the
+// cache's, at no cost; P's high and low parts take an instruction each. (O = P V
+// with the parts as rows took as many, but twice the accumulators: 8 warps per SM
+// for 16.) K and V in f32
+// are split too.
+template <typename T, int HD>
+__global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas)
+    attend_kernel(const AttendArgs a, const Scratch sc) {
+    using S = Shape<T, HD>;
+    constexpr int W = S::kWarps, kSlots = S::kSlots, kTiles = S::kTiles, kTile = S::kTile;
+    constexpr int kElems = 16 / (int)sizeof(T);  // of a 16-byte unit
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint8_t* ring = smem + warp * S::kUnits * S::kUnit;
+    // Eight neighbouring lanes copy a line: with the lines' quarters copied by lanes apart each was
+    // fetched from L2 twice (131071 slots, 64/8 heads of 128, bf16: 807 MB for 537, 111 us for 90).
+    // A row's 16-byte units lie in the ring exchanged within their line so that neither the copies (eight
+    // lanes a line) nor the reads (K: four lanes a row, two rows at a time; V: two units of four rows) meet
+    // in a bank: unit c of K row r at c ^ 4 (r % 2), of V row r at c ^ 2 (r / 2 % 4).
+    const uint32_t dst = smem_u32(ring) + (lane >> 3) * S::kRow;
+    const uint32_t k_dst = dst + ((lane & 7) ^ (((lane >> 3) & 1) * 4)) * 16;
+    const uint32_t v_dst[2] = {dst + ((lane & 7) ^ ((lane >> 4) * 2)) * 16,
+                               dst + ((lane & 7) ^ ((lane >> 4) * 2) ^ 4) * 16};
+    const uint8_t* k_src = ring + g * S::kRow + t * 16;
+    const int k_half[2] = {(g & 1) * 64, 64 - (g & 1) * 64};
+    const uint8_t* v_src = ring + 2 * t * S::kRow + (g ^ (2 * t)) * 16;
+    uint8_t* qs = smem + W * S::kUnits * S::kUnit;
+    float2* ml_s = reinterpret_cast<float2*>(qs + S::kQBytes);        // [W][kHeadTile]
+    float* unit_s = reinterpret_cast<float*>(ml_s + W * kHeadTile);   // [kHeadTile]
+    const int group = a.nq / a.kv.nkv;
+    const int heads = a.kv.nkv * sc.head_tiles;  // head tiles of a sequence
+
+    pdl_launch_dependents();
+
+    // my share: every warp adds up the sequences' steps by itself
+    const int B = a.kv.n_seqs, per = (B + 31) / 32;
+    int64_t mine = 0;
+    auto units_of = [&](const Slots& q) { return q.tiles ? (int64_t)(q.tiles + S::kSetup) * heads : 0; };
+    for (int b = lane * per; b < min(B, (lane + 1) * per); ++b) mine += units_of(slots_of<kSlots>(a, b));
+    int64_t before = mine;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        qr[j] = j < per ? q[lane + 32 * j] : 0.0f;
-        acc[j] = 0.0f;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += u;
     }
-    // l is summed with its rounding error carried in c: tens of thousands of
-    // small weights beside a large one would each round to nothing
-    float m = -INFINITY, l = 0.0f, c = 0.0f;
-    float* srow = scores ? scores + ((int64_t)b * a.nq + h) * a.kv.capacity() : nullptr;
-    for (int64_t t = first + warp; t < n; t += kWarps) {
-        const int64_t row = a.kv.row(b, kvh, t);
-        if (row < 0) {
-            if (srow && lane == 0) srow[t] = -INFINITY;
-            continue;
+    const int64_t total = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    int64_t share = (total + gridDim.x - 1) / gridDim.x;
+    if (share < S::kSetup + W) share = S::kSetup + W;  // a step a warp at least
+    const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
+    if (begin >= end) return;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, begin >= before && begin < before + mine)) - 1;
+    int b = owner * per;
+    int64_t off = begin - __shfl_sync(0xffffffffu, before, owner);
+    Slots s = slots_of<kSlots>(a, b);
+    while (off >= units_of(s)) {
+        off -= units_of(s);
+        s = slots_of<kSlots>(a, ++b);
+    }
+    int h = (int)(off / (s.tiles + S::kSetup));
+    // where the steps of (b, h) begin in the list
+    int64_t base = begin - (off - (int64_t)h * (s.tiles + S::kSetup)) + S::kSetup;
+
+    while (base < end) {
+        const int tile = (int)max(begin - base, (int64_t)0);
+        const int count = (int)min(end - base, (int64_t)s.tiles) - tile;  // at least 1: see the step to the next
+        const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * kHeadTile;
+        const int nh = min(kHeadTile, group - q0);
+        const int head0 = kvh * group + q0;
+        const int* table = a.kv.table + b * a.kv.table_stride;
+        const int mask = (1 << a.kv.page_shift) - 1;
+        const int my = count > warp ? (count - warp + W - 1) / W : 0;  // steps of this warp
+        const int my_slot0 = (s.tile0 + tile + warp) * kSlots;         // step i starts at slot my_slot0 + i W kSlots
+
+        // The pages of a step's tiles (a tile lies in one page), -1: none.
+        struct Pages {
+            int p[kTiles];
+        };
+        auto pages_of = [&](int i) {
+            Pages r;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) {
+                const int slot = my_slot0 + i * (W * kSlots) + u * kTile;
+                r.p[u] = i < my && slot < s.n ? table[slot >> a.kv.page_shift] : -1;
+            }
+            return r;
+        };
+        // Copies step i's rows of K (or V) into a unit of the ring; zeros where a slot is not seen.
+        auto issue = [&](int i, const Pages& pages, const void* pool, int unit, bool is_v) {
+            if (i < my) {
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u) {
+                    const int slot0 = my_slot0 + i * (W * kSlots) + u * kTile;
+                    const int page = pages.p[u];
+                    const bool ok = page >= 0 && page < a.kv.n_pages;
+                    const T* rows = static_cast<const T*>(pool) + ((ok ? page : 0) * a.kv.page_stride +
+                                                                   kvh * a.kv.head_stride +
+                                                                   (slot0 & mask) * a.kv.slot_stride);
+                    // four rows' 128-byte lines an instruction, a line by eight neighbouring lanes
+#pragma unroll
+                    for (int r = 0; r < kTile / 4; ++r) {
+                        const int row = 4 * r + (lane >> 3);
+                        const T* src = rows + row * a.kv.slot_stride + (lane & 7) * kElems;
+                        const bool live = ok && slot0 + row >= s.first && slot0 + row < s.n;
+                        const uint32_t dst = (is_v ? v_dst[r & 1] : k_dst) + unit * S::kUnit +
+                                             (u * kTile + 4 * r) * S::kRow;
+#pragma unroll
+                        for (int j = 0; j < S::kLines; ++j) copy16(dst + j * 128, src + j * 8 * kElems, live);
+                    }
+                }
+            }
+            copy_commit();
+        };
+        // K of step i is issued a step ahead, V half a step later, their page numbers half a step before
+        Pages pages = pages_of(0);
+        issue(0, pages, a.kv.k, 0, false);
+        issue(0, pages, a.kv.v, 1, true);
+        Pages seen = pages;
+        pages = pages_of(1);
+
+        // Q of the head tile in the order of operand A, its power of two taken out
+        for (int j = warp; j < kHeadTile; j += W) {
+            const float* q = a.q + b * a.ldq + (int64_t)(head0 + j) * HD;
+            float x[HD / 32], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                x[i] = j < nh ? q[lane + 32 * i] : 0.0f;
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            top = warp_max(top);
+            int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+            e = max(-126, min(126, e));
+            const float down = exp2f((float)-e);
+            if (lane == 0) unit_s[j] = a.scale * kLog2e * exp2f((float)e);
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                const int d = lane + 32 * i, c = d / kElems, r = d % kElems;
+                const int step = (c >> 2) * 2 + r / (kElems / 2), p = r % (kElems / 2);
+                T hi, lo;
+                split<T>(x[i] * down, &hi, &lo);
+                T* dst = reinterpret_cast<T*>(qs + (step * 32 + j * 4 + (c & 3)) * 16);
+                if constexpr (sizeof(T) == 4) {
+                    dst[2 * p] = hi;
+                    dst[2 * p + 1] = lo;
+                } else {
+                    dst[(p >> 1) * 4 + (p & 1)] = hi;
+                    dst[(p >> 1) * 4 + 2 + (p & 1)] = lo;
+                }
+            }
         }
-        const T* k = static_cast<const T*>(a.kv.k) + row;
-        const T* v = static_cast<const T*>(a.kv.v) + row;
-        float s = 0.0f;
+        __syncthreads();
+        const float unit = unit_s[g];
+        const uint8_t* qs_l = qs + lane * 16;
+        uint4 qr[S::kQRegs ? 2 * S::kChunks : 1];
+        if constexpr (S::kQRegs) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < per) s = fmaf(qr[j], kv_to_f32(k[lane + 32 * j]), s);
-        s = warp_sum(s) * a.scale;
-        if (srow && lane == 0) srow[t] = s;
-        const float m2 = fmaxf(m, s);
-        const float f = m2 == -INFINITY ? 1.0f : expf(m - m2);
-        const float p = m2 == -INFINITY ? 0.0f : expf(s - m2);
-        m = m2;
-        l *= f;
-        c = fmaf(c, f, p);
-        const float l2 = l + c;
-        c -= l2 - l;
-        l = l2;
+            for (int j = 0; j < 2 * S::kChunks; ++j) qr[j] = lds16(qs_l + j * 512);
+        }
+        float* srow = sc.scores && g < nh ? sc.scores + ((int64_t)b * a.nq + head0 + g) * a.kv.capacity() : nullptr;
+
+        float m = -INFINITY, l = 0.0f, lc = 0.0f;
+        float acc[HD / 16][4];  // [two columns]: head 2 t, head 2 t + 1 at the first; the same at the second
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < per) acc[j] = acc[j] * f + p * kv_to_f32(v[lane + 32 * j]);
+        for (int i = 0; i < HD / 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+
+        int at = 0;  // the unit of K of step i; V follows
+        for (int i = 0; i < my; ++i) {
+            const int at_v = at == 2 ? 0 : at + 1, spare = at_v == 2 ? 0 : at_v + 1;
+            copy_wait<1>();
+            __syncwarp();  // the other lanes' copies have landed too, and they have read the spare unit
+            issue(i + 1, pages, a.kv.k, spare, false);
+            const Pages after = pages_of(i + 2);
+            const uint8_t* src = k_src + at * S::kUnit;
+            // scores: two chains of products per 8 slots
+            constexpr int kX = kSlots / 4;
+            float x[kX];
+#pragma unroll
+            for (int r = 0; r < kSlots / 8; ++r) {
+                float c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < S::kChunks; ++j) {
+                    const uint4 k = lds16(src + 8 * r * S::kRow + (j >> 1) * 128 + k_half[j & 1]);
+                    uint4 qa, qb;
+                    if constexpr (S::kQRegs) qa = qr[2 * j], qb = qr[2 * j + 1];
+                    else qa = lds16(qs_l + (2 * j) * 512), qb = lds16(qs_l + (2 * j + 1) * 512);
+                    if constexpr (sizeof(T) == 4) {
+                        float hi[4], lo[4];
+                        split<T>(__uint_as_float(k.x), &hi[0], &lo[0]);
+                        split<T>(__uint_as_float(k.y), &hi[1], &lo[1]);
+                        split<T>(__uint_as_float(k.z), &hi[2], &lo[2]);
+                        split<T>(__uint_as_float(k.w), &hi[3], &lo[3]);
+                        mma<T>(c0, qa, __float_as_uint(hi[0]), __float_as_uint(hi[1]));
+                        mma<T>(c1, qb, __float_as_uint(hi[2]), __float_as_uint(hi[3]));
+                        mma<T>(c0, qa, __float_as_uint(lo[0]), __float_as_uint(lo[1]));
+                        mma<T>(c1, qb, __float_as_uint(lo[2]), __float_as_uint(lo[3]));
+                    } else {
+                        mma<T>(c0, qa, k.x, k.y);
+                        mma<T>(c1, qb, k.z, k.w);
+                    }
+                }
+                x[2 * r] = ((c0[0] + c1[0]) + (c0[2] + c1[2])) * unit;
+                x[2 * r + 1] = ((c0[1] + c1[1]) + (c0[3] + c1[3])) * unit;
+            }
+            // lane (g, t) has the scores of head g at slots 2 t, 2 t + 1 of every eight
+            const int slot0 = my_slot0 + i * (W * kSlots);
+            bool whole = slot0 >= s.first && slot0 + kSlots <= s.n;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) whole = whole && seen.p[u] >= 0 && seen.p[u] < a.kv.n_pages;
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < kX; ++r) {
+                    const int slot = slot0 + 2 * t + (r & 1) + 8 * (r >> 1);
+                    const int page = seen.p[r * 4 / kTile];
+                    if (page < 0 || page >= a.kv.n_pages || slot < s.first || slot >= s.n) x[r] = -INFINITY;
+                }
+            }
+            if (srow) {
+#pragma unroll
+                for (int r = 0; r < kX; ++r) {
+                    const int slot = slot0 + 2 * t + (r & 1) + 8 * (r >> 1);
+                    if (slot >= s.first && slot < s.n) srow[slot] = x[r];
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int r = 1; r < kX; ++r) top = fmaxf(top, x[r]);
+            top = quad_max(top);
+            if (__any_sync(0xffffffffu, top > m + kSlack<T>)) {
+                const float up = fmaxf(m, top), f = up == -INFINITY ? 1.0f : ex2(m - up);
+                const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    acc[j][0] *= f0;
+                    acc[j][1] *= f1;
+                    acc[j][2] *= f0;
+                    acc[j][3] *= f1;
+                }
+                l *= f;
+                lc *= f;
+                m = up;
+            }
+            const float zero = m == -INFINITY ? 0.0f : m - kWeightBias<T>;
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kX; ++r) {
+                x[r] = ex2(x[r] - zero);
+                sum += x[r];
+            }
+            // the rounding error of the sum is carried along: many small weights beside a large one count
+            lc += sum;
+            const float l2 = l + lc;
+            lc -= l2 - l;
+            l = l2;
+            uint4 p[kTiles];  // operand B: high parts x, y, low parts z, w
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) {
+                if constexpr (sizeof(T) == 4) {
+                    float hi[2], lo[2];
+                    split<T>(x[2 * u], &hi[0], &lo[0]);
+                    split<T>(x[2 * u + 1], &hi[1], &lo[1]);
+                    p[u] = make_uint4(__float_as_uint(hi[0]), __float_as_uint(hi[1]), __float_as_uint(lo[0]),
+                                      __float_as_uint(lo[1]));
+                } else {
+                    split2<T>(x[4 * u], x[4 * u + 1], &p[u].x, &p[u].z);
+                    split2<T>(x[4 * u + 2], x[4 * u + 3], &p[u].y, &p[u].w);
+                }
+            }
+            copy_wait<1>();
+            __syncwarp();  // every lane has read K's unit
+            issue(i + 1, pages, a.kv.v, at, true);
+            seen = pages;
+            pages = after;
+            src = v_src + at_v * S::kUnit;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                for (int j = 0; j < S::kLines; ++j) {
+                    uint4 v[S::kVRows];
+#pragma unroll
+                    for (int r = 0; r < S::kVRows; ++r)
+                        v[r] = lds16(src + (u * kTile + (r & 1) + 8 * (r >> 1)) * S::kRow + j * 128);
+                    const uint32_t v0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, v1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+                    if constexpr (sizeof(T) == 4) {
+                        // high V with both parts of P, low V with the high one: the rest is below 2^-22
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float hi[4], lo[4];
+                            split<T>(__uint_as_float(v0[2 * e]), &hi[0], &lo[0]);
+                            split<T>(__uint_as_float(v0[2 * e + 1]), &hi[1], &lo[1]);
+                            split<T>(__uint_as_float(v1[2 * e]), &hi[2], &lo[2]);
+                            split<T>(__uint_as_float(v1[2 * e + 1]), &hi[3], &lo[3]);
+                            const uint4 vh = make_uint4(__float_as_uint(hi[0]), __float_as_uint(hi[1]),
+                                                        __float_as_uint(hi[2]), __float_as_uint(hi[3]));
+                            const uint4 vl = make_uint4(__float_as_uint(lo[0]), __float_as_uint(lo[1]),
+                                                        __float_as_uint(lo[2]), __float_as_uint(lo[3]));
+                            mma<T>(acc[j * 2 + e], vh, p[u].x, p[u].y);
+                            mma<T>(acc[j * 2 + e], vl, p[u].x, p[u].y);
+                            mma<T>(acc[j * 2 + e], vh, p[u].z, p[u].w);
+                        }
+                    } else {
+                        const uint32_t v2[4] = {v[2].x, v[2].y, v[2].z, v[2].w};
+                        const uint32_t v3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint4 vv = make_uint4(__byte_perm(v0[e], v1[e], 0x5410),
+                                                        __byte_perm(v0[e], v1[e], 0x7632),
+                                                        __byte_perm(v2[e], v3[e], 0x5410),
+                                                        __byte_perm(v2[e], v3[e], 0x7632));
+                            mma<T>(acc[j * 4 + e], vv, p[u].x, p[u].y);
+                            mma<T>(acc[j * 4 + e], vv, p[u].z, p[u].w);
+                        }
+                    }
+                }
+            at = spare;
+        }
+        copy_wait<0>();
+
+        // the warps' results, each in its own ring: heads 2 t, 2 t + 1, the columns of the lane's V units
+        float* mine_s = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int j = 0; j < S::kLines; ++j)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < kElems; e += 4) {
+                    const int i = (j * kElems + e) / 2;
+                    *reinterpret_cast<float4*>(mine_s + (2 * t + half) * S::kAccRow + (j * 8 + g) * kElems + e) =
+                        make_float4(acc[i][half], acc[i][2 + half], acc[i + 1][half], acc[i + 1][2 + half]);
+                }
+        l = quad_sum(l + lc);
+        if (t == 0) ml_s[warp * kHeadTile + g] = make_float2(m, l);
+        __syncthreads();
+        const bool begins = tile == 0, ends = tile + count == s.tiles;
+        const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
+        if (begins && threadIdx.x == 0) {
+            const int64_t last = (base + s.tiles - 1) / share;
+            sc.plans[(int64_t)b * heads + h] = Plan{(int)blockIdx.x, (int)(last - blockIdx.x) + 1};
+        }
+        for (int i = threadIdx.x; i < nh * (HD / 4); i += W * 32) {
+            const int j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) M = fmaxf(M, ml_s[w * kHeadTile + j].x);
+            float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float2 ml = ml_s[w * kHeadTile + j];
+                const float f = piece_factor(ml.x, M);
+                L += ml.y * f;
+                const float4 p = *reinterpret_cast<const float4*>(
+                    reinterpret_cast<const float*>(smem + w * S::kUnits * S::kUnit) + j * S::kAccRow + d);
+                o.x += p.x * f;
+                o.y += p.y * f;
+                o.z += p.z * f;
+                o.w += p.w * f;
+            }
+            if (begins && ends) {
+                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+                *reinterpret_cast<float4*>(a.out + ((int64_t)b * a.nq + head0 + j) * HD + d) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                if (sc.stats && d == 0) sc.stats[(int64_t)b * a.nq + head0 + j] = make_float2(M, exp2f(-kWeightBias<T>) * L);
+            } else {
+                *reinterpret_cast<float4*>(sc.acc + ((int64_t)slot * kHeadTile + j) * HD + d) = o;
+                if (d == 0) sc.ml[slot * kHeadTile + j] = make_float2(M, L);
+            }
+        }
+        base += s.tiles + S::kSetup;
+        if (base >= end) return;
+        if (++h == heads) {
+            h = 0;
+            do s = slots_of<kSlots>(a, ++b);
+            while (s.tiles == 0);
+        }
+        __syncthreads();  // the rings and Q are rewritten
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < per) acc_s[warp][lane + 32 * j] = acc[j];
-    if (lane == 0) {
-        m_s[warp] = m;
-        l_s[warp] = l;
+}
+
+// Joins the pieces of divided (sequence, head tile)s in the order of the CTAs
+// that left them, and writes the zeros of sequences without slots. A CTA takes
+// kHeads heads of a head tile: one (blockIdx.y-th) where there are few head tiles
+// with many pieces, all eight where there are many. A thread sums four columns
+// of a head over every kGroups-th piece.
+template <int HD, int kHeads>
+struct JoinShape {
+    static constexpr int kCols = HD / 4;
+    static constexpr int kThreads = kHeads * kCols < 256 ? 256 : kHeads * kCols;
+    static constexpr int kGroups = kThreads / (kHeads * kCols);
+};
+template <int HD, int kSlots, int kHeads>
+__global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
+    join_kernel(const AttendArgs a, const Scratch sc, int max_pieces, float bias) {
+    using J = JoinShape<HD, kHeads>;
+    constexpr int kCols = J::kCols, kGroups = J::kGroups, kWarps = J::kThreads / 32;
+    extern __shared__ float factors[];  // [kHeads][max_pieces]
+    __shared__ float4 part[kGroups][kHeads][kCols];
+    __shared__ float2 ml_s[kHeads];
+    pdl_wait();
+    const int heads = a.kv.nkv * sc.head_tiles;
+    const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
+    const int group = a.nq / a.kv.nkv;
+    const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * kHeadTile;
+    const int nh = min(kHeadTile, group - q0);
+    const int j0 = blockIdx.y * kHeads;
+    if (j0 >= nh) return;
+    const int64_t head0 = (int64_t)b * a.nq + kvh * group + q0;
+    const int unit = threadIdx.x / kCols, col = threadIdx.x - unit * kCols;
+    const int grp = unit / kHeads, j = j0 + unit - grp * kHeads;
+    float4* out = reinterpret_cast<float4*>(a.out + (head0 + j) * HD) + col;
+    if (slots_of<kSlots>(a, b).tiles == 0) {
+        if (grp == 0 && j < nh) *out = make_float4(0, 0, 0, 0);
+        return;
+    }
+    const Plan plan = sc.plans[(int64_t)b * heads + h];
+    if (plan.pieces == 1) return;  // written by its CTA
+    auto slot = [&](int p) { return (int64_t)(p == 0 ? 2 * plan.first_cta + 1 : 2 * (plan.first_cta + p)); };
+    // a warp per head: the factors e^(m - M) and the sum, kept in piece order by the strides
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = warp; i < kHeads && j0 + i < nh; i += kWarps) {
+        float M = -INFINITY, L = 0.0f;
+        for (int p = lane; p < plan.pieces; p += 32) M = fmaxf(M, sc.ml[slot(p) * kHeadTile + j0 + i].x);
+        M = warp_max(M);
+        for (int p = lane; p < plan.pieces; p += 32) {
+            const float2 ml = sc.ml[slot(p) * kHeadTile + j0 + i];
+            const float f = piece_factor(ml.x, M);
+            factors[i * max_pieces + p] = f;
+            L += ml.y * f;
+        }
+        L = warp_sum(L);
+        if (lane == 0) {
+            ml_s[i] = make_float2(M, L);
+            if (sc.stats) sc.stats[head0 + j0 + i] = make_float2(M, exp2f(-bias) * L);
+        }
     }
     __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, m_s[w]);
-    float f[kWarps];
-    for (int w = 0; w < kWarps; ++w) {
-        f[w] = m_s[w] == -INFINITY ? 0.0f : expf(m_s[w] - M);
-        L += l_s[w] * f[w];
+    float4 o = make_float4(0, 0, 0, 0);
+    if (grp < kGroups && j < nh) {
+        const float* f = factors + (j - j0) * max_pieces;
+#pragma unroll 8
+        for (int p = grp; p < plan.pieces; p += kGroups) {
+            const float4 v = reinterpret_cast<const float4*>(sc.acc + (slot(p) * kHeadTile + j) * HD)[col];
+            o.x += v.x * f[p];
+            o.y += v.y * f[p];
+            o.z += v.z * f[p];
+            o.w += v.w * f[p];
+        }
+        part[grp][j - j0][col] = o;
     }
-    for (int d = threadIdx.x; d < hd; d += kThreads) {
-        float s = 0.0f;
-        for (int w = 0; w < kWarps; ++w) s += acc_s[w][d] * f[w];
-        a.out[((int64_t)b * a.nq + h) * hd + d] = L > 0.0f ? s / L : 0.0f;
+    if constexpr (kGroups > 1) __syncthreads();
+    if (grp > 0 || j >= nh) return;
+#pragma unroll
+    for (int q = 1; q < kGroups; ++q) {
+        const float4 v = part[q][j - j0][col];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
     }
-    if (stats && threadIdx.x == 0) stats[(int64_t)b * a.nq + h] = make_float2(M, L);
+    const float L = ml_s[j - j0].y, inv = L > 0.0f ? 1.0f / L : 0.0f;
+    *out = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // weights_out[b][kv][t] = weights[b][kv][t] + sum over the kv head's query heads of the slot's weight.
-__global__ void __launch_bounds__(kThreads) weights_kernel(const AttendArgs a, const float* scores,
-                                                           const float2* stats) {
+constexpr int kWeightThreads = 256;
+__global__ void __launch_bounds__(kWeightThreads) weights_kernel(const AttendArgs a, const Scratch sc) {
     const int kvh = blockIdx.y, b = blockIdx.z;
     const int64_t cap = a.kv.capacity();
-    const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t t = (int64_t)blockIdx.x * kWeightThreads + threadIdx.x;
     if (t >= cap) return;
-    int64_t first, n;
-    slot_range(a, b, &first, &n);
+    const Slots s = slots_of<16>(a, b);
     const int64_t at = ((int64_t)b * a.kv.nkv + kvh) * cap + t;
     float w = a.weights[at];
-    if (t >= first && t < n) {
+    if (t >= s.first && t < s.n) {
         const int g = a.nq / a.kv.nkv;
         float p = 0.0f;
         for (int j = 0; j < g; ++j) {
             const int64_t h = (int64_t)b * a.nq + kvh * g + j;
-            const float2 ml = stats[h];
-            if (ml.y > 0.0f) p += expf(scores[h * cap + t] - ml.x) / ml.y;
+            const float2 ml = sc.stats[h];
+            if (ml.y > 0.0f) p += exp2f(sc.scores[h * cap + t] - ml.x) / ml.y;
         }
         w += p;
     }
     a.weights_out[at] = w;
 }
 
+int head_tiles(const PagedKv& kv, int nq) { return (nq / kv.nkv + kHeadTile - 1) / kHeadTile; }
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        return 148;
+    return sms;
+}
+
+constexpr int kMaxCtas = 2;  // per SM, of any shape
+size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Carves the workspace; returns its size.
+size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Scratch* sc) {
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        void* p = static_cast<uint8_t*>(base) + off;
+        off += aligned(bytes);
+        return p;
+    };
+    sc->head_tiles = head_tiles(kv, nq);
+    sc->plans = static_cast<Plan*>(take((size_t)kv.n_seqs * kv.nkv * sc->head_tiles * sizeof(Plan)));
+    sc->ml = static_cast<float2*>(take((size_t)grid * 2 * kHeadTile * sizeof(float2)));
+    sc->acc = static_cast<float*>(take((size_t)grid * 2 * kHeadTile * kv.hd * sizeof(float)));
+    sc->stats = nullptr;
+    sc->scores = nullptr;
+    if (weights) {
+        sc->stats = static_cast<float2*>(take((size_t)kv.n_seqs * nq * sizeof(float2)));
+        sc->scores = static_cast<float*>(take((size_t)kv.n_seqs * nq * kv.capacity() * sizeof(float)));
+    }
+    return off;
+}
+
+template <typename T, int HD>
+cudaError_t launch(const AttendArgs& a, const Scratch& sc, int sms, cudaStream_t st) {
+    using S = Shape<T, HD>;
+    const void* fn = (const void*)attend_kernel<T, HD>;
+    cudaError_t e = ensure_dynamic_smem(fn, S::kSmem);
+    if (e != cudaSuccess) return e;
+    const int grid = sms * S::kCtas;
+    attend_kernel<T, HD><<<grid, S::kWarps * 32, S::kSmem, st>>>(a, sc);
+    note_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const int tiles = a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
+    const int heads = a.nq / a.kv.nkv < kHeadTile ? a.nq / a.kv.nkv : kHeadTile;
+    int pieces = grid;
+    float bias = kWeightBias<T>;
+    AttendArgs aa = a;
+    Scratch ss = sc;
+    void* args[] = {&aa, &ss, &pieces, &bias};
+    // few head tiles: their heads side by side
+    if (tiles * heads <= 8 * sms)
+        return launch_pdl_kernel((const void*)join_kernel<HD, S::kSlots, 1>, dim3(tiles, heads),
+                                 dim3(JoinShape<HD, 1>::kThreads), grid * sizeof(float), st, args);
+    return launch_pdl_kernel((const void*)join_kernel<HD, S::kSlots, kHeadTile>, dim3(tiles),
+                             dim3(JoinShape<HD, kHeadTile>::kThreads), kHeadTile * grid * sizeof(float), st, args);
+}
+
+template <typename T>
+cudaError_t launch_hd(const AttendArgs& a, const Scratch& sc, int sms, cudaStream_t st) {
+    switch (a.kv.hd) {
+        case 64: return launch<T, 64>(a, sc, sms, st);
+        case 128: return launch<T, 128>(a, sc, sms, st);
+        case 192: return launch<T, 192>(a, sc, sms, st);
+        case 256: return launch<T, 256>(a, sc, sms, st);
+    }
+    return cudaErrorInvalidValue;
+}
+
 }  // namespace
 
 size_t paged_attention_workspace(const PagedKv& kv, int nq, bool weights) {
-    if (!weights) return 0;
-    return (size_t)kv.n_seqs * nq * (sizeof(float2) + (size_t)kv.capacity() * sizeof(float));
+    Scratch sc;
+    return carve(kv, nq, weights, sm_count() * kMaxCtas, nullptr, &sc);
 }
 
 cudaError_t launch_paged_attention(const AttendArgs& a, void* ws, cudaStream_t st) {
     if (a.kv.n_seqs <= 0) return cudaSuccess;
-    float2* stats = nullptr;
-    float* scores = nullptr;
-    if (a.weights) {
-        stats = static_cast<float2*>(ws);
-        scores = reinterpret_cast<float*>(stats + (size_t)a.kv.n_seqs * a.nq);
+    const int sms = sm_count();
+    Scratch sc;
+    carve(a.kv, a.nq, a.weights != nullptr, sms * kMaxCtas, ws, &sc);
+    cudaError_t e = cudaErrorInvalidValue;
+    switch (a.kv.dtype) {
+        case kKvF32: e = launch_hd<float>(a, sc, sms, st); break;
+        case kKvF16: e = launch_hd<__half>(a, sc, sms, st); break;
+        case kKvBF16: e = launch_hd<__nv_bfloat16>(a, sc, sms, st); break;
     }
-    const dim3 grid(a.nq, a.kv.n_seqs);
-    if (a.kv.dtype == kKvF32) attend_kernel<float><<<grid, kThreads, 0, st>>>(a, scores, stats);
-    else if (a.kv.dtype == kKvF16) attend_kernel<__half><<<grid, kThreads, 0, st>>>(a, scores, stats);
-    else attend_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, scores, stats);
-    note_launch();
-    cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !a.weights) return e;
-    const dim3 wgrid((unsigned)((a.kv.capacity() + kThreads - 1) / kThreads), a.kv.nkv, a.kv.n_seqs);
-    weights_kernel<<<wgrid, kThreads, 0, st>>>(a, scores, stats);
+    const dim3 wgrid((unsigned)((a.kv.capacity() + kWeightThreads - 1) / kWeightThreads), a.kv.nkv, a.kv.n_seqs);
+    weights_kernel<<<wgrid, kWeightThreads, 0, st>>>(a, sc);
     note_launch();
     return cudaGetLastError();
 }
