@@ -1142,7 +1142,8 @@ QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, 
             return fail(QMM_ERR_INVALID_INPUT, "null pointer");
         if (ld_q < (size_t)n_heads * a.kv.hd || window < 0)
             return fail(QMM_ERR_SHAPE_MISMATCH, "query row stride or window out of range");
-        if (!aligned16(q_dev) || ld_q % 4 || !aligned16(out_dev))
+        if (!aligned16(q_dev) || ld_q % 4 || !aligned16(out_dev) || !aligned16(weights_dev) ||
+            !aligned16(weights_out_dev))
             return fail(QMM_ERR_INVALID_INPUT, "misaligned pointer (16 B) or row stride (4 floats)");
         a.q = q_dev;
         a.ldq = (int64_t)ld_q;

@@ -141,25 +141,67 @@ __device__ __forceinline__ Slots slots_of(const AttendArgs& a, int b) {
     return s;
 }
 
-// A piece of the work: consecutive tiles of one (sequence, head tile). The
-// list of all (sequence, head tile)s, each kSetup units of starting and ending it
-// followed by one unit per tile, is cut into equal shares, one per CTA (without
-// the setup's units a CTA got dozens of short sequences where another had part
-// of one: 64 sequences of 1 to 8192 slots, 64/8 heads of 128, f16 took 238 us
-// instead of 101). Pieces that are not a whole (sequence, head tile) leave (acc, m, l)
-// behind: in the CTA's slot 0 if earlier CTAs hold the beginning, in slot 1 if not.
-struct Plan {
-    int first_cta, pieces;  // of a (sequence, head tile)
-};
-
+// The list of all (sequence, head tile)s -- each kSetup units for starting and
+// ending it, then one unit per step -- is cut into equal shares, one per CTA.
+// (Without the setup's units a CTA got dozens of short sequences where another
+// had part of one: 64 sequences of 1 to 8192 slots, 64/8 heads of 128, f16 took
+// 238 us instead of 101.) A piece is a CTA's part of a (sequence, head tile); one
+// that is not the whole leaves (acc, m, l) behind: in the CTA's slot 0 if earlier
+// CTAs hold the beginning, in slot 1 if not.
 struct Scratch {
-    Plan* plans;     // [n_seqs][head tiles]
-    float2* ml;      // [grid][2][kHeadTile]: maximum (in units of log 2) and sum of a piece
+    float2* ml;      // [grid][2][kHeadTile]: reference and sum of a piece (see kSlack)
     float* acc;      // [grid][2][kHeadTile][hd]
-    float2* stats;   // [n_seqs][nq], with weights: the final maximum and sum
+    float2* whole;   // [n_seqs][nq], with weights: the same of undivided head tiles
     float* scores;   // [n_seqs][nq][capacity], with weights: scores in units of log 2
     int head_tiles;  // per kv head
+    int grid;        // CTAs of attend_kernel
 };
+
+// Units of all sequences (total) and of those before `seq` (before); each lane
+// of a warp adds up a run of B / 32 sequences.
+template <typename S>
+__device__ __forceinline__ int64_t units_of(const Slots& s, int heads) {
+    return s.tiles ? (int64_t)(s.tiles + S::kSetup) * heads : 0;
+}
+// Units per CTA; a step per warp at least.
+template <typename S>
+__device__ __forceinline__ int64_t share_of(int64_t total, int grid) {
+    const int64_t share = (total + grid - 1) / grid, least = S::kSetup + S::kWarps;
+    return share < least ? least : share;
+}
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The CTAs that hold the pieces of (sequence b, head tile h).
+struct Pieces {
+    int first, count;
+    // Slot of piece p among the CTAs' slots.
+    __device__ __forceinline__ int64_t slot(int p) const { return p == 0 ? 2 * first + 1 : 2 * (first + p); }
+};
+struct Place {
+    int64_t start, share;  // unit at which the sequence starts, units per CTA
+    int tiles;
+    template <typename S>
+    __device__ __forceinline__ Pieces pieces(int h) const {
+        const int64_t base = start + (int64_t)h * (tiles + S::kSetup) + S::kSetup;
+        const int64_t first = base / share, last = (base + tiles - 1) / share;
+        return Pieces{(int)first, (int)(last - first) + 1};
+    }
+};
+template <typename S>
+__device__ __forceinline__ Place place_of(const AttendArgs& a, const Scratch& sc, int b) {
+    const int heads = a.kv.nkv * sc.head_tiles;
+    int64_t total = 0, before = 0;
+    for (int i = threadIdx.x & 31; i < a.kv.n_seqs; i += 32) {
+        const int64_t u = units_of<S>(slots_of<S::kSlots>(a, i), heads);
+        total += u;
+        if (i < b) before += u;
+    }
+    return Place{warp_sum64(before), share_of<S>(warp_sum64(total), sc.grid), slots_of<S::kSlots>(a, b).tiles};
+}
 
 // kTile slots are the K of one instruction's P; a step takes kTiles of them. A
 // warp's ring holds three units of a step's K or V rows: one in use, two on
@@ -178,7 +220,7 @@ struct Shape {
     static constexpr int kUnits = 3;
     static constexpr int kWarps = HD <= 128 ? 8 : (HD <= 192 ? 5 : 4);
     static constexpr int kCtas = 2;                              // per SM
-    static constexpr int kSetup = 65536 / (2 * kUnit);           // a piece's fixed cost in steps: about 3 us
+    static constexpr int kSetup = 163840 / (2 * kUnit);          // a piece's fixed cost in steps: 6 us measured
     static constexpr int kQBytes = kChunks * 2 * 32 * 16;
     static constexpr bool kQRegs = kChunks <= (kWarps == 8 ? 4 : 8);  // Q in registers
     static constexpr int kAccRow = HD + 4;                       // floats; spreads the rows over the banks
@@ -244,8 +286,7 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
     // my share: every warp adds up the sequences' steps by itself
     const int B = a.kv.n_seqs, per = (B + 31) / 32;
     int64_t mine = 0;
-    auto units_of = [&](const Slots& q) { return q.tiles ? (int64_t)(q.tiles + S::kSetup) * heads : 0; };
-    for (int b = lane * per; b < min(B, (lane + 1) * per); ++b) mine += units_of(slots_of<kSlots>(a, b));
+    for (int b = lane * per; b < min(B, (lane + 1) * per); ++b) mine += units_of<S>(slots_of<kSlots>(a, b), heads);
     int64_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -254,16 +295,15 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
     }
     const int64_t total = __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
-    int64_t share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < S::kSetup + W) share = S::kSetup + W;  // a step a warp at least
+    const int64_t share = share_of<S>(total, gridDim.x);
     const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
     if (begin >= end) return;
     const int owner = __ffs(__ballot_sync(0xffffffffu, begin >= before && begin < before + mine)) - 1;
     int b = owner * per;
     int64_t off = begin - __shfl_sync(0xffffffffu, before, owner);
     Slots s = slots_of<kSlots>(a, b);
-    while (off >= units_of(s)) {
-        off -= units_of(s);
+    while (off >= units_of<S>(s, heads)) {
+        off -= units_of<S>(s, heads);
         s = slots_of<kSlots>(a, ++b);
     }
     int h = (int)(off / (s.tiles + S::kSetup));
@@ -541,10 +581,6 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
         __syncthreads();
         const bool begins = tile == 0, ends = tile + count == s.tiles;
         const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-        if (begins && threadIdx.x == 0) {
-            const int64_t last = (base + s.tiles - 1) / share;
-            sc.plans[(int64_t)b * heads + h] = Plan{(int)blockIdx.x, (int)(last - blockIdx.x) + 1};
-        }
         for (int i = threadIdx.x; i < nh * (HD / 4); i += W * 32) {
             const int j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
             float M = -INFINITY, L = 0.0f;
@@ -567,7 +603,7 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
                 const float inv = L > 0.0f ? 1.0f / L : 0.0f;
                 *reinterpret_cast<float4*>(a.out + ((int64_t)b * a.nq + head0 + j) * HD + d) =
                     make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-                if (sc.stats && d == 0) sc.stats[(int64_t)b * a.nq + head0 + j] = make_float2(M, exp2f(-kWeightBias<T>) * L);
+                if (sc.whole && d == 0) sc.whole[(int64_t)b * a.nq + head0 + j] = make_float2(M, L);
             } else {
                 *reinterpret_cast<float4*>(sc.acc + ((int64_t)slot * kHeadTile + j) * HD + d) = o;
                 if (d == 0) sc.ml[slot * kHeadTile + j] = make_float2(M, L);
@@ -589,106 +625,176 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
 // kHeads heads of a head tile: one (blockIdx.y-th) where there are few head tiles
 // with many pieces, all eight where there are many. A thread sums four columns
 // of a head over every kGroups-th piece.
-template <int HD, int kHeads>
+// It is on the way of every small call, so it is launched early (programmatic
+// dependent launch), finds the pieces from the lengths before it waits for
+// attend_kernel, and has one round of loads after it.
+// With weights, the CTAs from join_blocks on add the slots' weights.
+template <typename T, int HD, int kHeads>
 struct JoinShape {
     static constexpr int kCols = HD / 4;
     static constexpr int kThreads = kHeads * kCols < 256 ? 256 : kHeads * kCols;
     static constexpr int kGroups = kThreads / (kHeads * kCols);
+    static constexpr int kAhead = 4;        // pieces a thread loads before their factors are known
+    static constexpr int kHeadsAtOnce = 32;  // of a weights CTA
 };
-template <int HD, int kSlots, int kHeads>
-__global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
-    join_kernel(const AttendArgs a, const Scratch sc, int max_pieces, float bias) {
-    using J = JoinShape<HD, kHeads>;
-    constexpr int kCols = J::kCols, kGroups = J::kGroups, kWarps = J::kThreads / 32;
-    extern __shared__ float factors[];  // [kHeads][max_pieces]
-    __shared__ float4 part[kGroups][kHeads][kCols];
-    __shared__ float2 ml_s[kHeads];
+
+// weights_out[b][kvh][t] = weights[b][kvh][t] + sum over the kv head's query
+// heads of e^(s_t - m) / sum e^(s - m), four slots a thread.
+template <typename T, int HD, int kThreads, int kHeadsAtOnce>
+__device__ __forceinline__ void add_weights(const AttendArgs& a, const Scratch& sc, int64_t block) {
+    using S = Shape<T, HD>;
+    __shared__ float2 zero_inv[kHeadsAtOnce];  // what to subtract from a score, what to multiply its power with
+    const int64_t cap = a.kv.capacity();
+    const int64_t blocks = (cap / 4 + kThreads - 1) / kThreads;  // of a (sequence, kv head)
+    const int64_t row = block / blocks;
+    const int b = (int)(row / a.kv.nkv), kvh = (int)(row - (int64_t)b * a.kv.nkv);
+    const int64_t t = ((block - row * blocks) * kThreads + threadIdx.x) * 4;
+    const Place place = place_of<S>(a, sc, b);
+    const Slots s = slots_of<S::kSlots>(a, b);
+    const int64_t at = row * cap + t;
+    const bool mine = t < cap && t < s.n && t + 4 > s.first;
+    const bool copy = t < cap && !mine && a.weights_out != a.weights;
+    float4 w = make_float4(0, 0, 0, 0);
+    if (mine || copy) w = *reinterpret_cast<const float4*>(a.weights + at);
+    if (copy) *reinterpret_cast<float4*>(a.weights_out + at) = w;
     pdl_wait();
+    if (s.tiles == 0) return;
+    const int group = a.nq / a.kv.nkv;
+    const int64_t head0 = (int64_t)b * a.nq + kvh * group;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float p[4] = {0, 0, 0, 0};
+    for (int g0 = 0; g0 < group; g0 += kHeadsAtOnce) {
+        const int heads = min(kHeadsAtOnce, group - g0);
+        if (g0) __syncthreads();
+        for (int i = warp; i < heads; i += kThreads / 32) {
+            const int j = g0 + i;
+            const Pieces pc = place.pieces<S>(kvh * sc.head_tiles + j / kHeadTile);
+            float M = -INFINITY, L = 0.0f;
+            if (pc.count == 1) {
+                const float2 ml = sc.whole[head0 + j];
+                M = ml.x;
+                L = ml.y;
+            } else {
+                for (int q = lane; q < pc.count; q += 32) M = fmaxf(M, sc.ml[pc.slot(q) * kHeadTile + j % kHeadTile].x);
+                M = warp_max(M);
+                for (int q = lane; q < pc.count; q += 32) {
+                    const float2 ml = sc.ml[pc.slot(q) * kHeadTile + j % kHeadTile];
+                    L += ml.y * piece_factor(ml.x, M);
+                }
+                L = warp_sum(L);
+            }
+            if (lane == 0) zero_inv[i] = L > 0.0f ? make_float2(M - kWeightBias<T>, 1.0f / L) : make_float2(0.0f, 0.0f);
+        }
+        __syncthreads();
+        if (mine) {
+#pragma unroll 4
+            for (int i = 0; i < heads; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(sc.scores + (head0 + g0 + i) * cap + t);
+                const float2 z = zero_inv[i];
+                if (z.y > 0.0f) {
+                    p[0] += ex2(x.x - z.x) * z.y;
+                    p[1] += ex2(x.y - z.x) * z.y;
+                    p[2] += ex2(x.z - z.x) * z.y;
+                    p[3] += ex2(x.w - z.x) * z.y;
+                }
+            }
+        }
+    }
+    if (!mine) return;
+    auto in = [&](int i) { return t + i >= s.first && t + i < s.n; };  // scores elsewhere were not written
+    if (in(0)) w.x += p[0];
+    if (in(1)) w.y += p[1];
+    if (in(2)) w.z += p[2];
+    if (in(3)) w.w += p[3];
+    *reinterpret_cast<float4*>(a.weights_out + at) = w;
+}
+
+template <typename T, int HD, int kHeads>
+__global__ void __launch_bounds__(JoinShape<T, HD, kHeads>::kThreads)
+    join_kernel(const AttendArgs a, const Scratch sc, unsigned join_blocks) {
+    using S = Shape<T, HD>;
+    using J = JoinShape<T, HD, kHeads>;
+    constexpr int kCols = J::kCols, kGroups = J::kGroups, kWarps = J::kThreads / 32, kAhead = J::kAhead;
+    extern __shared__ float factors[];  // [kHeads][grid]
+    __shared__ float4 part[kGroups][kHeads][kCols];
+    __shared__ float inv_s[kHeads];
+    if (blockIdx.x >= join_blocks) {
+        if (blockIdx.y == 0) add_weights<T, HD, J::kThreads, J::kHeadsAtOnce>(a, sc, blockIdx.x - join_blocks);
+        else pdl_wait();
+        return;
+    }
     const int heads = a.kv.nkv * sc.head_tiles;
     const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
     const int group = a.nq / a.kv.nkv;
     const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * kHeadTile;
-    const int nh = min(kHeadTile, group - q0);
-    const int j0 = blockIdx.y * kHeads;
-    if (j0 >= nh) return;
-    const int64_t head0 = (int64_t)b * a.nq + kvh * group + q0;
+    const int j0 = blockIdx.y * kHeads, nh = min(kHeads, min(kHeadTile, group - q0) - j0);
+    const int64_t head0 = (int64_t)b * a.nq + kvh * group + q0 + j0;
     const int unit = threadIdx.x / kCols, col = threadIdx.x - unit * kCols;
-    const int grp = unit / kHeads, j = j0 + unit - grp * kHeads;
+    const int grp = unit / kHeads, j = unit - grp * kHeads;
+    const Place place = place_of<S>(a, sc, b);
+    const Pieces pc = place.pieces<S>(h);
+    pdl_wait();
+    if (nh <= 0) return;
     float4* out = reinterpret_cast<float4*>(a.out + (head0 + j) * HD) + col;
-    if (slots_of<kSlots>(a, b).tiles == 0) {
+    if (place.tiles == 0) {
         if (grp == 0 && j < nh) *out = make_float4(0, 0, 0, 0);
         return;
     }
-    const Plan plan = sc.plans[(int64_t)b * heads + h];
-    if (plan.pieces == 1) return;  // written by its CTA
-    auto slot = [&](int p) { return (int64_t)(p == 0 ? 2 * plan.first_cta + 1 : 2 * (plan.first_cta + p)); };
-    // a warp per head: the factors e^(m - M) and the sum, kept in piece order by the strides
+    if (pc.count == 1) return;  // written by its CTA
+    const bool mine = grp < kGroups && j < nh;
+    auto load = [&](int p) {
+        return reinterpret_cast<const float4*>(sc.acc + (pc.slot(p) * kHeadTile + j0 + j) * HD)[col];
+    };
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (mine && grp + i * kGroups < pc.count) ahead[i] = load(grp + i * kGroups);
+    // a warp per head: the factors e^(m - M) and the sum
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = warp; i < kHeads && j0 + i < nh; i += kWarps) {
-        float M = -INFINITY, L = 0.0f;
-        for (int p = lane; p < plan.pieces; p += 32) M = fmaxf(M, sc.ml[slot(p) * kHeadTile + j0 + i].x);
+    for (int i = warp; i < nh; i += kWarps) {
+        const float2* ml = sc.ml + j0 + i;
+        float2 first = lane < pc.count ? ml[pc.slot(lane) * kHeadTile] : make_float2(-INFINITY, 0.0f);
+        float M = first.x, L = 0.0f;
+        for (int p = lane + 32; p < pc.count; p += 32) M = fmaxf(M, ml[pc.slot(p) * kHeadTile].x);
         M = warp_max(M);
-        for (int p = lane; p < plan.pieces; p += 32) {
-            const float2 ml = sc.ml[slot(p) * kHeadTile + j0 + i];
-            const float f = piece_factor(ml.x, M);
-            factors[i * max_pieces + p] = f;
-            L += ml.y * f;
+        for (int p = lane; p < pc.count; p += 32) {
+            const float2 v = p == lane ? first : ml[pc.slot(p) * kHeadTile];
+            const float f = piece_factor(v.x, M);
+            factors[i * sc.grid + p] = f;
+            L += v.y * f;
         }
         L = warp_sum(L);
-        if (lane == 0) {
-            ml_s[i] = make_float2(M, L);
-            if (sc.stats) sc.stats[head0 + j0 + i] = make_float2(M, exp2f(-bias) * L);
-        }
+        if (lane == 0) inv_s[i] = L > 0.0f ? 1.0f / L : 0.0f;
     }
     __syncthreads();
     float4 o = make_float4(0, 0, 0, 0);
-    if (grp < kGroups && j < nh) {
-        const float* f = factors + (j - j0) * max_pieces;
-#pragma unroll 8
-        for (int p = grp; p < plan.pieces; p += kGroups) {
-            const float4 v = reinterpret_cast<const float4*>(sc.acc + (slot(p) * kHeadTile + j) * HD)[col];
+    if (mine) {
+        const float* f = factors + j * sc.grid;
+        auto add = [&](const float4& v, int p) {
             o.x += v.x * f[p];
             o.y += v.y * f[p];
             o.z += v.z * f[p];
             o.w += v.w * f[p];
-        }
-        part[grp][j - j0][col] = o;
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (grp + i * kGroups < pc.count) add(ahead[i], grp + i * kGroups);
+#pragma unroll 8
+        for (int p = grp + kAhead * kGroups; p < pc.count; p += kGroups) add(load(p), p);
+        part[grp][j][col] = o;
     }
     if constexpr (kGroups > 1) __syncthreads();
     if (grp > 0 || j >= nh) return;
 #pragma unroll
     for (int q = 1; q < kGroups; ++q) {
-        const float4 v = part[q][j - j0][col];
+        const float4 v = part[q][j][col];
         o.x += v.x;
         o.y += v.y;
         o.z += v.z;
         o.w += v.w;
     }
-    const float L = ml_s[j - j0].y, inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const float inv = inv_s[j];
     *out = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-}
-
-// weights_out[b][kv][t] = weights[b][kv][t] + sum over the kv head's query heads of the slot's weight.
-constexpr int kWeightThreads = 256;
-__global__ void __launch_bounds__(kWeightThreads) weights_kernel(const AttendArgs a, const Scratch sc) {
-    const int kvh = blockIdx.y, b = blockIdx.z;
-    const int64_t cap = a.kv.capacity();
-    const int64_t t = (int64_t)blockIdx.x * kWeightThreads + threadIdx.x;
-    if (t >= cap) return;
-    const Slots s = slots_of<16>(a, b);
-    const int64_t at = ((int64_t)b * a.kv.nkv + kvh) * cap + t;
-    float w = a.weights[at];
-    if (t >= s.first && t < s.n) {
-        const int g = a.nq / a.kv.nkv;
-        float p = 0.0f;
-        for (int j = 0; j < g; ++j) {
-            const int64_t h = (int64_t)b * a.nq + kvh * g + j;
-            const float2 ml = sc.stats[h];
-            if (ml.y > 0.0f) p += exp2f(sc.scores[h * cap + t] - ml.x) / ml.y;
-        }
-        w += p;
-    }
-    a.weights_out[at] = w;
 }
 
 int head_tiles(const PagedKv& kv, int nq) { return (nq / kv.nkv + kHeadTile - 1) / kHeadTile; }
@@ -713,42 +819,45 @@ size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Scra
         return p;
     };
     sc->head_tiles = head_tiles(kv, nq);
-    sc->plans = static_cast<Plan*>(take((size_t)kv.n_seqs * kv.nkv * sc->head_tiles * sizeof(Plan)));
     sc->ml = static_cast<float2*>(take((size_t)grid * 2 * kHeadTile * sizeof(float2)));
     sc->acc = static_cast<float*>(take((size_t)grid * 2 * kHeadTile * kv.hd * sizeof(float)));
-    sc->stats = nullptr;
+    sc->whole = nullptr;
     sc->scores = nullptr;
     if (weights) {
-        sc->stats = static_cast<float2*>(take((size_t)kv.n_seqs * nq * sizeof(float2)));
+        sc->whole = static_cast<float2*>(take((size_t)kv.n_seqs * nq * sizeof(float2)));
         sc->scores = static_cast<float*>(take((size_t)kv.n_seqs * nq * kv.capacity() * sizeof(float)));
     }
     return off;
 }
 
+template <typename T, int HD, int kHeads>
+cudaError_t launch_join(AttendArgs a, Scratch sc, int grid_y, cudaStream_t st) {
+    using J = JoinShape<T, HD, kHeads>;
+    unsigned join_blocks = (unsigned)(a.kv.n_seqs * a.kv.nkv * sc.head_tiles);
+    int64_t blocks = join_blocks;
+    if (a.weights)
+        blocks += (int64_t)a.kv.n_seqs * a.kv.nkv * ((a.kv.capacity() / 4 + J::kThreads - 1) / J::kThreads);
+    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    void* args[] = {&a, &sc, &join_blocks};
+    return launch_pdl_kernel((const void*)join_kernel<T, HD, kHeads>, dim3((unsigned)blocks, grid_y),
+                             dim3(J::kThreads), kHeads * sc.grid * sizeof(float), st, args);
+}
+
 template <typename T, int HD>
-cudaError_t launch(const AttendArgs& a, const Scratch& sc, int sms, cudaStream_t st) {
+cudaError_t launch(const AttendArgs& a, Scratch sc, int sms, cudaStream_t st) {
     using S = Shape<T, HD>;
-    const void* fn = (const void*)attend_kernel<T, HD>;
-    cudaError_t e = ensure_dynamic_smem(fn, S::kSmem);
+    cudaError_t e = ensure_dynamic_smem((const void*)attend_kernel<T, HD>, S::kSmem);
     if (e != cudaSuccess) return e;
-    const int grid = sms * S::kCtas;
-    attend_kernel<T, HD><<<grid, S::kWarps * 32, S::kSmem, st>>>(a, sc);
+    sc.grid = sms * S::kCtas;
+    attend_kernel<T, HD><<<sc.grid, S::kWarps * 32, S::kSmem, st>>>(a, sc);
     note_launch();
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int tiles = a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
     const int heads = a.nq / a.kv.nkv < kHeadTile ? a.nq / a.kv.nkv : kHeadTile;
-    int pieces = grid;
-    float bias = kWeightBias<T>;
-    AttendArgs aa = a;
-    Scratch ss = sc;
-    void* args[] = {&aa, &ss, &pieces, &bias};
     // few head tiles: their heads side by side
-    if (tiles * heads <= 8 * sms)
-        return launch_pdl_kernel((const void*)join_kernel<HD, S::kSlots, 1>, dim3(tiles, heads),
-                                 dim3(JoinShape<HD, 1>::kThreads), grid * sizeof(float), st, args);
-    return launch_pdl_kernel((const void*)join_kernel<HD, S::kSlots, kHeadTile>, dim3(tiles),
-                             dim3(JoinShape<HD, kHeadTile>::kThreads), kHeadTile * grid * sizeof(float), st, args);
+    if ((int64_t)tiles * heads <= 8 * sms) return launch_join<T, HD, 1>(a, sc, heads, st);
+    return launch_join<T, HD, kHeadTile>(a, sc, 1, st);
 }
 
 template <typename T>
@@ -774,17 +883,12 @@ cudaError_t launch_paged_attention(const AttendArgs& a, void* ws, cudaStream_t s
     const int sms = sm_count();
     Scratch sc;
     carve(a.kv, a.nq, a.weights != nullptr, sms * kMaxCtas, ws, &sc);
-    cudaError_t e = cudaErrorInvalidValue;
     switch (a.kv.dtype) {
-        case kKvF32: e = launch_hd<float>(a, sc, sms, st); break;
-        case kKvF16: e = launch_hd<__half>(a, sc, sms, st); break;
-        case kKvBF16: e = launch_hd<__nv_bfloat16>(a, sc, sms, st); break;
+        case kKvF32: return launch_hd<float>(a, sc, sms, st);
+        case kKvF16: return launch_hd<__half>(a, sc, sms, st);
+        case kKvBF16: return launch_hd<__nv_bfloat16>(a, sc, sms, st);
     }
-    if (e != cudaSuccess || !a.weights) return e;
-    const dim3 wgrid((unsigned)((a.kv.capacity() + kWeightThreads - 1) / kWeightThreads), a.kv.nkv, a.kv.n_seqs);
-    weights_kernel<<<wgrid, kWeightThreads, 0, st>>>(a, sc);
-    note_launch();
-    return cudaGetLastError();
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace qmm

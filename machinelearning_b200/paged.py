@@ -20,6 +20,7 @@ one dense f32 cache per sequence (layers/main/src/core/attention.rs:454-610).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -28,6 +29,9 @@ from . import _lib
 from ._lib import KV_BF16, KV_F16, KV_F32
 
 KV_DTYPES = {torch.float32: KV_F32, torch.float16: KV_F16, torch.bfloat16: KV_BF16}
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _mismatch(message: str) -> _lib.ShapeMismatch:
@@ -52,6 +56,7 @@ class PagedKVCache:
             raise _mismatch("rows of the cache and of the block table have to be contiguous")
         self.k, self.v, self.block_table = k, v, block_table
         self.device = k.device
+        self._index = k.device.index
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.n_seqs, self.max_pages = block_table.shape
         self.capacity = self.max_pages * self.page_size  # slots of one sequence
@@ -62,6 +67,7 @@ class PagedKVCache:
                                   self.max_pages, block_table.stride(0) if self.n_seqs > 1 else self.max_pages)
         self._ref = ctypes.byref(self._desc)
         self._lib = _lib.lib()
+        self._seqs_shape = (self.n_seqs,)
         self._slots_shape = (self.n_seqs, self.n_kv_heads, self.capacity)
 
     @classmethod
@@ -74,24 +80,23 @@ class PagedKVCache:
         table = torch.arange(n_seqs * per, dtype=torch.int32, device=dev).view(n_seqs, per)
         return cls(k, torch.zeros_like(k), table)
 
-    # ---- argument checks ---------------------------------------------------------------
-    def _check(self, t: torch.Tensor, name: str, dtype: torch.dtype, shape=None) -> int:
-        """The pointer of a contiguous tensor of this type (and shape) on the cache's device."""
-        if t.dtype != dtype:
+    # ---- argument checks (a few attribute reads a tensor: small steps are bound by the host) ----
+    def _check(self, t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> int:
+        """The pointer of a contiguous tensor of this type and shape on the cache's device."""
+        if t.dtype is dtype and t.shape == shape and t.get_device() == self._index and t.is_contiguous():
+            return t.data_ptr()
+        if t.dtype is not dtype:
             raise _lib.DTypeMismatch(_lib.ERR_DTYPE_MISMATCH, f"{name}: {t.dtype}, expected {dtype}")
-        if shape is not None and t.shape != shape:
+        if t.shape != shape:
             raise _mismatch(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if t.device != self.device or not t.is_contiguous():
-            raise ValueError(f"{name} has to be contiguous and on {self.device}")
-        return t.data_ptr()
+        raise ValueError(f"{name} has to be contiguous and on {self.device}")
 
-    def _rows(self, t: torch.Tensor, name: str):
-        """(pointer, row stride) of an f32 tensor whose rows are contiguous."""
-        if t.dtype != torch.float32:
+    def _rows(self, t: torch.Tensor, name: str, row: int):
+        """(pointer, row stride) of an f32 tensor of contiguous rows of ``row`` values."""
+        if t.dtype is not torch.float32:
             raise _lib.DTypeMismatch(_lib.ERR_DTYPE_MISMATCH, f"{name}: {t.dtype}, expected torch.float32")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name} has to be on {self.device}")
-        row = t.numel() // t.shape[0] if t.shape[0] else 0
         if t.is_contiguous():
             return t.data_ptr(), row
         if t[0].is_contiguous():
@@ -99,12 +104,13 @@ class PagedKVCache:
         raise ValueError(f"{name}: rows have to be contiguous")
 
     def _call(self, fn, *args) -> None:
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        if torch.cuda.current_device() == self.device.index:
-            _lib.check(fn(self._ref, *args, stream))
-        else:
-            with torch.cuda.device(self.device):
-                _lib.check(fn(self._ref, *args, stream))
+        status = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(self._index))
+        if status:
+            _lib.check(status)
+
+    def _on_device(self):
+        """The library launches on the current device: a context that makes it the cache's."""
+        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)
 
     # ---- operators ---------------------------------------------------------------------
     def append(self, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, cos: torch.Tensor,
@@ -117,27 +123,26 @@ class PagedKVCache:
         sequence ``seqs[i]`` (default: sequence i). ``positions[i]`` picks the row of
         the cos/sin tables [ctx][head_dim / 2]. Rows with slot -1 store nothing."""
         tokens, hd = qkv.shape[0], self.head_dim
-        if qkv.numel() != tokens * (n_heads + 2 * self.n_kv_heads) * hd:
+        row = (n_heads + 2 * self.n_kv_heads) * hd
+        if qkv.numel() != tokens * row:
             raise _mismatch(f"qkv: {tuple(qkv.shape)} is not [tokens][({n_heads} + 2 * {self.n_kv_heads}) * {hd}]")
-        if cos.dim() != 2 or cos.shape[1] * 2 != hd:
-            raise _mismatch(f"cos: {tuple(cos.shape)} is not [ctx][{hd // 2}]")
+        ctx = cos.shape[0]
         if seqs is None and tokens > self.n_seqs:
             raise _mismatch(f"{tokens} tokens for {self.n_seqs} sequences: seqs is needed")
         if (q_norm is None) != (k_norm is None):
             raise ValueError("q_norm and k_norm: both or neither")
-        i32, f32 = torch.int32, torch.float32
-        ptr, ld = self._rows(qkv, "qkv")
-        shape = (tokens, n_heads, hd)
-        if out is None:
-            out = torch.empty(shape, dtype=f32, device=self.device)
-        self._call(self._lib.qmm_paged_append_dev, ptr, ld, tokens, n_heads,
-                   None if q_norm is None else self._check(q_norm, "q_norm", f32, (hd,)),
-                   None if k_norm is None else self._check(k_norm, "k_norm", f32, (hd,)), offset, eps,
-                   self._check(cos, "cos", f32), self._check(sin, "sin", f32, cos.shape), cos.shape[0],
-                   int(interleaved), self._check(positions, "positions", i32, (tokens,)),
-                   self._check(slots, "slots", i32, (tokens,)),
-                   None if seqs is None else self._check(seqs, "seqs", i32, (tokens,)),
-                   self._check(out, "out", f32, shape))
+        i32, f32, check, one = torch.int32, torch.float32, self._check, (tokens,)
+        ptr, ld = self._rows(qkv, "qkv", row)
+        shape, table = (tokens, n_heads, hd), (ctx, hd // 2)
+        with self._on_device():
+            if out is None:
+                out = torch.empty(shape, dtype=f32, device=self.device)
+            self._call(self._lib.qmm_paged_append_dev, ptr, ld, tokens, n_heads,
+                       None if q_norm is None else check(q_norm, "q_norm", f32, (hd,)),
+                       None if k_norm is None else check(k_norm, "k_norm", f32, (hd,)), offset, eps,
+                       check(cos, "cos", f32, table), check(sin, "sin", f32, table), ctx, int(interleaved),
+                       check(positions, "positions", i32, one), check(slots, "slots", i32, one),
+                       None if seqs is None else check(seqs, "seqs", i32, one), check(out, "out", f32, shape))
         return out
 
     def attend(self, q: torch.Tensor, lengths: torch.Tensor, scale: float, *, window: int = 0,
@@ -148,21 +153,23 @@ class PagedKVCache:
         them, 0: all); a sequence of length 0 gives zeros. ``weights`` f32
         [sequences][kv heads][capacity]: every slot's softmax weight, summed over
         the kv head's query heads, is added (into ``weights_out`` if given)."""
-        if q.dim() != 3 or q.shape[0] != self.n_seqs or q.shape[2] != self.head_dim:
-            raise _mismatch(f"q: {tuple(q.shape)} is not [{self.n_seqs}][heads][{self.head_dim}]")
-        f32 = torch.float32
-        ptr, ld = self._rows(q, "q")
-        if out is None:
-            out = torch.empty(q.shape, dtype=f32, device=self.device)
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != self.n_seqs or shape[2] != self.head_dim:
+            raise _mismatch(f"q: {tuple(shape)} is not [{self.n_seqs}][heads][{self.head_dim}]")
+        f32, check = torch.float32, self._check
+        ptr, ld = self._rows(q, "q", shape[1] * shape[2])
         w = w_out = None
         if weights is not None:
-            w = self._check(weights, "weights", f32, self._slots_shape)
-            w_out = w if weights_out is None else self._check(weights_out, "weights_out", f32, self._slots_shape)
+            w = check(weights, "weights", f32, self._slots_shape)
+            w_out = w if weights_out is None else check(weights_out, "weights_out", f32, self._slots_shape)
         elif weights_out is not None:
             raise ValueError("weights_out without weights")
-        self._call(self._lib.qmm_paged_attention_dev, ptr, ld, q.shape[1],
-                   self._check(lengths, "lengths", torch.int32, (self.n_seqs,)), scale, int(window), w, w_out,
-                   self._check(out, "out", f32, q.shape))
+        with self._on_device():
+            if out is None:
+                out = torch.empty(shape, dtype=f32, device=self.device)
+            self._call(self._lib.qmm_paged_attention_dev, ptr, ld, shape[1],
+                       check(lengths, "lengths", torch.int32, self._seqs_shape), scale, window, w, w_out,
+                       check(out, "out", f32, shape))
         return out
 
     def evict(self, lengths: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor,
@@ -173,13 +180,13 @@ class PagedKVCache:
         the lowest slot. Kept slots at or above ``budget`` move (k and v in place)
         into the evicted ones below it, in slot order. ``weights`` f32 and
         ``positions`` int32 [sequences][kv heads][capacity] are not changed."""
-        i32, f32 = torch.int32, torch.float32
-        new = (torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(positions))
-        self._call(self._lib.qmm_paged_evict_dev, self._check(lengths, "lengths", i32, (self.n_seqs,)),
-                   self._check(weights, "weights", f32, self._slots_shape),
-                   self._check(positions, "positions", i32, self._slots_shape),
-                   self._check(next_positions, "next_positions", i32, (self.n_seqs,)), int(budget), int(recent),
-                   new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr())
+        i32, f32, check, slots = torch.int32, torch.float32, self._check, self._slots_shape
+        args = (check(lengths, "lengths", i32, self._seqs_shape), check(weights, "weights", f32, slots),
+                check(positions, "positions", i32, slots),
+                check(next_positions, "next_positions", i32, self._seqs_shape), budget, recent)
+        with self._on_device():
+            new = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(positions)
+            self._call(self._lib.qmm_paged_evict_dev, *args, new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr())
         return new
 
     def reserve(self, n_heads: int, weights: bool = False, budget: int = 0,
