@@ -367,7 +367,7 @@ QMM_API int qmm_paged_append_dev(const qmm_paged_kv* kv, const float* qkv_dev, s
 /* One new token per sequence: out_dev [n_seqs][n_heads][head_dim] = softmax(scale
  * q . k) v over the sequence's slots [max(0, n - window), n), n = lengths_dev[s]
  * clamped to [0, capacity], window 0: all. A sequence without slots gives
- * zeros. q rows ld_q floats apart (a multiple of 4; 16-byte aligned pointers).
+ * zeros. q rows ld_q floats apart (a multiple of 4); float pointers 16-byte aligned.
  * weights_dev and weights_out_dev (both or neither; they may be equal), f32
  * [n_seqs][n_kv_heads][capacity]: out = in, plus at each attended slot the sum
  * over the kv head's query heads of the slot's softmax weight. Workspace: the
@@ -387,7 +387,8 @@ QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, 
  * at or above `budget` move, in slot order, into the evicted ones below it (k and
  * v in place); weights_out_dev and positions_out_dev (not the inputs) hold the
  * moved arrays, 0 and -1 beyond the new length; lengths_out_dev [n_seqs] (not
- * lengths_dev) the new lengths. Workspace as above. */
+ * lengths_dev) the new lengths. Weights and positions 16-byte aligned; at most
+ * 65535 (sequence, kv head) rows. Workspace as above. */
 QMM_API size_t qmm_paged_evict_workspace_size(const qmm_paged_kv* kv, int budget);
 QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, const float* weights_dev,
                                 const int* positions_dev, const int* next_positions_dev, int budget, int recent,

@@ -1181,6 +1181,11 @@ QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, 
             return fail(QMM_ERR_INVALID_INPUT, "null pointer");
         if (weights_out_dev == weights_dev || positions_out_dev == positions_dev || lengths_out_dev == lengths_dev)
             return fail(QMM_ERR_INVALID_INPUT, "eviction does not write its inputs: pass separate outputs");
+        if (!aligned16(weights_dev) || !aligned16(positions_dev) || !aligned16(weights_out_dev) ||
+            !aligned16(positions_out_dev))
+            return fail(QMM_ERR_INVALID_INPUT, "misaligned weights or positions (16 B)");
+        if ((long long)a.kv.n_seqs * a.kv.nkv > 65535)
+            return fail(QMM_ERR_SHAPE_MISMATCH, "more than 65535 (sequence, kv head) rows");
         if (budget < 1 || recent < 0 || recent > budget)
             return fail(QMM_ERR_SHAPE_MISMATCH, "budget below 1, or recent outside [0, budget]");
         a.lengths = lengths_dev;
