@@ -23,11 +23,11 @@ namespace qmm {
 namespace {
 
 constexpr int kSelectThreads = 1024;
-constexpr int kPer = 8;                    // consecutive slots of a thread in a round
-constexpr int kRound = kSelectThreads * kPer;    // slots a CTA takes in a round
-constexpr int kMaxCluster = 8;             // the portable size
+constexpr int kPer = 8;                        // consecutive slots of a thread in a round
+constexpr int kRound = kSelectThreads * kPer;  // slots a CTA takes in a round
+constexpr int kMaxCluster = 8;                 // the portable size
 constexpr int kDigits = 256;
-constexpr int kCopies = 8;                 // of a histogram: neighbouring lanes count in different ones
+constexpr int kCopies = 8;  // of a histogram: neighbouring lanes count in different ones
 
 // Unsigned order of the preference: a total order on the floats, protected
 // slots above all of them. w + 0 turns -0 into +0, its equal.
@@ -68,7 +68,8 @@ __device__ __forceinline__ int ld_cluster_s32(const int* local, uint32_t rank) {
 // budget, whichever is later (the holes end before); counts per row and CTA.
 struct Lists {
     int* list;     // [rows][capacity]
-    int2* counts;  // [rows][kMaxCluster]: holes, movers
+    int2* counts;  // [rows][ctas]: holes, movers
+    int rows;
     int ctas;      // per row
     int range;     // slots of a CTA, a multiple of kPer
 };
@@ -93,24 +94,24 @@ __device__ __forceinline__ Row row_of(const EvictArgs& a, int row) {
 // The threshold by four rounds of counting 8-bit digits, from the top: after
 // each, the digit of the budget-th preferred key among those that match the
 // digits so far. kCluster: the CTAs of a row count their ranges and add up each
-// other's counts through distributed shared memory.
-template <bool kCluster>
+// other's counts through distributed shared memory. kHeld: a CTA's range is one
+// round, whose slots stay in registers; longer ranges are read again (from L1 and
+// L2) each time.
+template <bool kCluster, bool kHeld>
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs a, const Lists ls) {
-    __shared__ int hist[kCopies][kDigits + 4];
-    __shared__ int counts[4][kDigits];  // of this CTA, per digit round
+    __shared__ __align__(16) int hist[2][kCopies][kDigits + 4];  // of this round and the next
+    __shared__ __align__(16) int counts[4][kDigits];             // of this CTA, per digit round
     __shared__ int warp_sums[32];
     __shared__ int s_digit, s_left;
+    pdl_launch_dependents();
     const int row = blockIdx.y, rank = kCluster ? (int)blockIdx.x : 0;
-    const Row r = row_of(a, row);
-    const int64_t cap = a.kv.capacity();
+    const int64_t cap = a.kv.capacity(), base = row * cap;
     const int begin = rank * ls.range, end = (int)min((int64_t)begin + ls.range, cap);
-    const int live = min(end, r.n);  // slots of mine that are cached: [begin, live)
-    const float* w = a.weights + r.base;
-    const int* pos = a.positions + r.base;
-    float* w_out = a.weights_out + r.base;
-    int* pos_out = a.positions_out + r.base;
-    if (rank == 0 && row % a.kv.nkv == 0 && threadIdx.x == 0) a.lengths_out[row / a.kv.nkv] = r.kept;
-    const int tid8 = threadIdx.x * kPer;
+    const float* w = a.weights + base;
+    const int* pos = a.positions + base;
+    float* w_out = a.weights_out + base;
+    int* pos_out = a.positions_out + base;
+    const int tid8 = threadIdx.x * kPer, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     struct Slots8 {
         float w[kPer];
@@ -130,32 +131,40 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
         *reinterpret_cast<int4*>(pos_out + t) = *reinterpret_cast<const int4*>(s.p);
         *reinterpret_cast<int4*>(pos_out + t + 4) = *reinterpret_cast<const int4*>(s.p + 4);
     };
+    Slots8 held = {};
+    if (kHeld && begin + tid8 < end) held = load(begin + tid8);  // beside the loads of row_of
+    auto slots = [&](int t) { return kHeld ? held : load(t); };
+    for (int i = threadIdx.x; i < kCopies * (kDigits + 4); i += kSelectThreads) (&hist[0][0][0])[i] = 0;
+
+    const Row r = row_of(a, row);
+    const int live = min(end, r.n);  // slots of mine that are cached: [begin, live)
+    if (rank == 0 && row % a.kv.nkv == 0 && threadIdx.x == 0) a.lengths_out[row / a.kv.nkv] = r.kept;
     // what lies beyond the kept slots, and all of a row that is short enough
     const bool full = r.n > a.budget;
     for (int t = begin + tid8; t < end; t += kRound) {
         if (full && t < r.kept) continue;
-        Slots8 s;
-        if (t < r.kept) s = load(t);
+        Slots8 s = {};
+        if (t < r.kept) s = slots(t);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
             if (t + i >= r.kept) s.w[i] = 0.0f, s.p[i] = -1;
-        if (!full || t >= r.kept) store(t, s);
+        store(t, s);
     }
+    int2* my_counts = ls.counts + (int64_t)row * ls.ctas + rank;
     if (!full) {
-        if (threadIdx.x == 0) ls.counts[(int64_t)row * kMaxCluster + rank] = make_int2(0, 0);
+        if (threadIdx.x == 0) *my_counts = make_int2(0, 0);
         return;
     }
+    __syncthreads();
 
     uint32_t prefix = 0;
     int need = a.budget;  // slots still to take among those that match the prefix
 #pragma unroll 1
     for (int round = 0; round < 4; ++round) {
         const int shift = 24 - 8 * round;
-        for (int i = threadIdx.x; i < kCopies * (kDigits + 4); i += kSelectThreads) (&hist[0][0])[i] = 0;
-        __syncthreads();
-        int* mine = hist[threadIdx.x & (kCopies - 1)];
+        int* mine = hist[round & 1][threadIdx.x & (kCopies - 1)];
         for (int t = begin + tid8; t < live; t += kRound) {
-            const Slots8 s = load(t);
+            const Slots8 s = slots(t);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const uint32_t key = slot_key(s.w[i], s.p[i] >= r.limit);
@@ -164,31 +173,47 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
             }
         }
         __syncthreads();
-        if (threadIdx.x < kDigits) {
-            int c = 0;
+        if constexpr (kCluster) {
+            if (threadIdx.x < kDigits) {
+                int c = 0;
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) c += hist[i][threadIdx.x];
-            counts[round][threadIdx.x] = c;
-        }
-        if constexpr (kCluster) cluster_sync();
-        else __syncthreads();
-        // thread i has digit 255 - i: the first whose running count reaches `need`
-        const int d = kDigits - 1 - (int)threadIdx.x;
-        int c = 0;
-        if (threadIdx.x < kDigits) {
-            if constexpr (kCluster) {
-#pragma unroll
-                for (int q = 0; q < kMaxCluster; ++q)
-                    if (q < ls.ctas) c += ld_cluster_s32(&counts[round][d], q);
-            } else {
-                c = counts[round][d];
+                for (int i = 0; i < kCopies; ++i) c += hist[round & 1][i][threadIdx.x];
+                counts[round][threadIdx.x] = c;
             }
+            cluster_sync();
         }
-        int total;
-        const int above = block_scan(c, warp_sums, &total);
-        if (threadIdx.x < kDigits && above < need && above + c >= need) {
-            s_digit = d;
-            s_left = need - above;
+        // the first warp finds the digit (lane l has digits 255 - 8 l down), the others clear for the next round
+        if (warp == 0) {
+            int c[8] = {};
+            const int d0 = kDigits - 8 - 8 * lane;
+            if constexpr (kCluster) {
+                for (int q = 0; q < ls.ctas; ++q)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) c[i] += ld_cluster_s32(&counts[round][d0 + i], q);
+            } else {
+#pragma unroll
+                for (int q = 0; q < kCopies; ++q) {
+                    const int4 lo = *reinterpret_cast<const int4*>(&hist[round & 1][q][d0]);
+                    const int4 hi = *reinterpret_cast<const int4*>(&hist[round & 1][q][d0 + 4]);
+                    c[0] += lo.x, c[1] += lo.y, c[2] += lo.z, c[3] += lo.w;
+                    c[4] += hi.x, c[5] += hi.y, c[6] += hi.z, c[7] += hi.w;
+                }
+            }
+            int sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += c[i];
+            int above = warp_scan(sum) - sum;
+            if (above < need && above + sum >= need) {  // one lane
+                int d = 7;
+#pragma unroll
+                for (int i = 7; i >= 0; --i)
+                    if (d == i && above + c[i] < need) above += c[i], d = i - 1;
+                s_digit = d0 + d;
+                s_left = need - above;
+            }
+        } else {
+            for (int i = threadIdx.x - 32; i < kCopies * (kDigits + 4); i += kSelectThreads - 32)
+                (&hist[(round + 1) & 1][0][0])[i] = 0;
         }
         __syncthreads();
         prefix |= (uint32_t)s_digit << shift;
@@ -200,15 +225,15 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
         for (int q = 0; q < rank; ++q) ties += ld_cluster_s32(&counts[3][prefix & (kDigits - 1)], q);
         cluster_sync();  // nobody reads my counts any more
     }
-    int* list = ls.list + r.base;
+    int* list = ls.list + base;
     const int first_mover = max(begin, a.budget);
     int holes = 0, movers = 0;
     for (int t0 = begin; t0 < live; t0 += kRound) {
         const int t = t0 + tid8;
-        Slots8 s;
+        Slots8 s = {};
         uint32_t tie = 0, keep = 0, in = 0;  // bit per slot
         if (t < live) {
-            s = load(t);
+            s = slots(t);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const uint32_t key = slot_key(s.w[i], s.p[i] >= r.limit);
@@ -247,68 +272,106 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
         // the holes' entries are move_kernel's: what is written to them here comes before
         if (t < live && t < r.kept) store(t, s);
     }
-    if (threadIdx.x == 0) ls.counts[(int64_t)row * kMaxCluster + rank] = make_int2(holes, movers);
+    if (threadIdx.x == 0) *my_counts = make_int2(holes, movers);
 }
 
-// A warp takes kBatch moves at a time: their slots and rows first, then all the
-// 16-byte units of their K and V rows, eight loads of a lane in flight.
+// The moves of all rows are dealt out in batches, warp by warp: a lane finds the
+// slots and rows of a move, then all lanes copy the 16-byte units of the batch's K
+// and V rows, eight loads of a lane in flight. The chain of loads before the copy
+// is paid once a batch, so there are no more batches than warps as long as a
+// batch is at most 32 moves (with batches of four, 16 sequences of 1500 to 8192
+// slots, 8 kv heads of 128, took 51 us instead of 23).
 constexpr int kMoveThreads = 256;
-constexpr int kBatch = 8;
-constexpr int kLoads = 8;
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictArgs a, const Lists ls, int units) {
-    const int row = blockIdx.x, lane = threadIdx.x & 31;
+constexpr int kMoveCtas = 3;  // per SM: one wave
+// kSteps: 16-byte units of a move (its K row, then its V row) per lane.
+template <int kSteps>
+__global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const EvictArgs a, const Lists ls, int units) {
+    constexpr int kMoves = 8 / kSteps;  // with their loads in flight together
+    const int lane = threadIdx.x & 31;
+    const int64_t cap = a.kv.capacity();
     pdl_wait();
-    const int2* counts = ls.counts + (int64_t)row * kMaxCluster;
-    int2 c = lane < ls.ctas ? counts[lane] : make_int2(0, 0);
-    const int2 through = make_int2(warp_scan(c.x), warp_scan(c.y));  // up to and with CTA `lane`
-    const int moves = __shfl_sync(0xffffffffu, through.x, 31);
-    const int b = row / a.kv.nkv, h = row - b * a.kv.nkv;
-    const int64_t base = row * a.kv.capacity();
-    const int warps = gridDim.y * (kMoveThreads / 32);
-    const int size16 = 2 * units;  // 16-byte units of a move: K's, then V's
-    const int bytes = units * 16 / a.kv.hd;
-    for (int i0 = (blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kBatch; i0 < moves; i0 += warps * kBatch) {
-        const int count = min(kBatch, moves - i0);
-        int64_t dst = -1, src = -1;
-        const int i = i0 + lane;
-        // the CTAs whose lists hold hole i and mover i
-        int qh = 0, qm = 0, before_h = 0, before_m = 0;
-        for (int q = 0; q < ls.ctas; ++q) {
-            const int th = __shfl_sync(0xffffffffu, through.x, q), tm = __shfl_sync(0xffffffffu, through.y, q);
-            if (i >= th) qh = q + 1, before_h = th;
-            if (i >= tm) qm = q + 1, before_m = tm;
+    // each lane adds up a run of rows
+    const int per = (ls.rows + 31) / 32, r0 = lane * per, r1 = min(ls.rows, r0 + per);
+    auto holes_of = [&](int row) {
+        int n = 0;
+        for (int q = 0; q < ls.ctas; ++q) n += ls.counts[(int64_t)row * ls.ctas + q].x;
+        return n;
+    };
+    const int64_t warps = (int64_t)gridDim.x * (kMoveThreads / 32);
+    int64_t mine = 0;
+    for (int row = r0; row < r1; ++row) mine += holes_of(row);
+    int64_t all_moves = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all_moves += __shfl_xor_sync(0xffffffffu, all_moves, o);
+    // of a batch: rows end with part of one, and a second batch for some warps would double the time
+    const int64_t deal = warps > 2 * ls.rows ? warps - ls.rows : warps;
+    const int size = (int)max((int64_t)1, min((all_moves + deal - 1) / deal, (int64_t)32));
+    mine = 0;
+    for (int row = r0; row < r1; ++row) mine += (holes_of(row) + size - 1) / size;
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += u;
+    }
+    const int64_t batches = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    const int bytes = units * 16 / a.kv.hd;  // of an element
+    char* unit_at[kSteps];                    // this lane's units of row 0; null: none
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const int u = lane + 32 * i;
+        unit_at[i] = u < units ? static_cast<char*>(a.kv.k) + u * 16
+                               : (u < 2 * units ? static_cast<char*>(a.kv.v) + (u - units) * 16 : nullptr);
+    }
+    for (int64_t k = (int64_t)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); k < batches; k += warps) {
+        const int owner = __ffs(__ballot_sync(0xffffffffu, k >= before && k < before + mine)) - 1;
+        int64_t batch = k - __shfl_sync(0xffffffffu, before, owner);
+        int row = owner * per, moves = holes_of(row);
+        while (batch >= (moves + size - 1) / size) {
+            batch -= (moves + size - 1) / size;
+            moves = holes_of(++row);
         }
+        const int count = min(size, moves - (int)batch * size);
+        const int b = row / a.kv.nkv, h = row - b * a.kv.nkv;
+        const int64_t base = row * cap;
+        int64_t dst = -1, src = -1;
         if (lane < count) {
-            const int to = ls.list[base + (int64_t)qh * ls.range + i - before_h];
-            const int of = ls.list[base + max(qm * ls.range, a.budget) + i - before_m];
+            const int i = (int)batch * size + lane;
+            // the CTAs whose lists hold hole i and mover i
+            int hole = 0, mover = 0, holes = 0, movers = 0;
+            for (int q = 0; q < ls.ctas; ++q) {
+                const int2 c = ls.counts[(int64_t)row * ls.ctas + q];
+                if (i >= holes && i < holes + c.x) hole = q * ls.range + i - holes;
+                if (i >= movers && i < movers + c.y) mover = max(q * ls.range, a.budget) + i - movers;
+                holes += c.x;
+                movers += c.y;
+            }
+            const int to = ls.list[base + hole], of = ls.list[base + mover];
             a.weights_out[base + to] = a.weights[base + of];
             a.positions_out[base + to] = a.positions[base + of];
             dst = a.kv.row(b, h, to);
             src = a.kv.row(b, h, of);
             if (dst < 0 || src < 0) dst = src = -1;  // a slot without a page has no row
         }
-        const int all = count * size16;
-        for (int u0 = 0; u0 < all; u0 += 32 * kLoads) {
-            uint4 v[kLoads];
-            char* to[kLoads];
+        for (int m0 = 0; m0 < count; m0 += kMoves) {
+            uint4 v[kMoves][kSteps];
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-                const int u = u0 + j * 32 + lane;
-                const int m = u < all ? u / size16 : 0;
-                const int64_t d = __shfl_sync(0xffffffffu, dst, m), s = __shfl_sync(0xffffffffu, src, m);
-                to[j] = nullptr;
-                if (u < all && d >= 0) {
-                    int part = u - m * size16;
-                    const bool is_v = part >= units;
-                    if (is_v) part -= units;
-                    char* pool = static_cast<char*>(is_v ? a.kv.v : a.kv.k) + part * 16;
-                    v[j] = *reinterpret_cast<const uint4*>(pool + s * bytes);
-                    to[j] = pool + d * bytes;
-                }
+            for (int m = 0; m < kMoves; ++m) {
+                const int64_t from = __shfl_sync(0xffffffffu, src, (m0 + m) & 31) * bytes;
+                if (m0 + m < count && from >= 0)
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i)
+                        if (unit_at[i]) v[m][i] = *reinterpret_cast<const uint4*>(unit_at[i] + from);
             }
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-                if (to[j]) *reinterpret_cast<uint4*>(to[j]) = v[j];
+            for (int m = 0; m < kMoves; ++m) {
+                const int64_t to = __shfl_sync(0xffffffffu, dst, (m0 + m) & 31) * bytes;
+                if (m0 + m < count && to >= 0)
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i)
+                        if (unit_at[i]) *reinterpret_cast<uint4*>(unit_at[i] + to) = v[m][i];
+            }
         }
     }
 }
@@ -341,6 +404,7 @@ cudaError_t launch_paged_evict(const EvictArgs& a0, void* ws, cudaStream_t st) {
     if (a.budget > cap) a.budget = (int)cap;  // no sequence is longer
     Lists ls;
     divide(a.kv, &ls);
+    ls.rows = (int)rows;
     ls.counts = static_cast<int2*>(ws);
     ls.list = reinterpret_cast<int*>(static_cast<uint8_t*>(ws) + aligned(rows * kMaxCluster * sizeof(int2)));
 
@@ -355,21 +419,22 @@ cudaError_t launch_paged_evict(const EvictArgs& a0, void* ws, cudaStream_t st) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ls.ctas > 1 ? 1 : 0;
-    cudaError_t e = ls.ctas > 1 ? cudaLaunchKernelEx(&cfg, select_kernel<true>, a, ls)
-                                : cudaLaunchKernelEx(&cfg, select_kernel<false>, a, ls);
+    cudaError_t e;
+    if (ls.ctas == 1) e = cudaLaunchKernelEx(&cfg, select_kernel<false, true>, a, ls);
+    else if (ls.range <= kRound) e = cudaLaunchKernelEx(&cfg, select_kernel<true, true>, a, ls);
+    else e = cudaLaunchKernelEx(&cfg, select_kernel<true, false>, a, ls);
     note_launch();
     if (e != cudaSuccess) return e;
 
-    // enough warps for every move of every row, up to 8 CTAs per SM
-    int64_t most = a.budget < cap - a.budget ? a.budget : cap - a.budget;
-    const int64_t per_cta = kMoveThreads / 32 * kBatch;
-    int64_t y = (most + per_cta - 1) / per_cta;
-    const int64_t enough = (148 * 8 + rows - 1) / rows;
-    if (y > enough) y = enough;
-    if (y < 1) y = 1;
+    // a warp for every move there can be, one wave at most
+    const int64_t most = rows * (a.budget < cap - a.budget ? a.budget : cap - a.budget) + 1;
+    int64_t grid = (most + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
+    if (grid > 148 * kMoveCtas) grid = 148 * kMoveCtas;
     int units = a.kv.hd * kv_type_size(a.kv.dtype) / 16;
     void* args[] = {&a, &ls, &units};
-    return launch_pdl_kernel((const void*)move_kernel, dim3((unsigned)rows, (unsigned)y), dim3(kMoveThreads), 0, st, args);
+    const void* fn[] = {(const void*)move_kernel<1>, (const void*)move_kernel<2>, (const void*)move_kernel<4>,
+                        (const void*)move_kernel<4>};
+    return launch_pdl_kernel(fn[(2 * units + 31) / 32 - 1], dim3((unsigned)grid), dim3(kMoveThreads), 0, st, args);
 }
 
 }  // namespace qmm
