@@ -1092,9 +1092,7 @@ QMM_API int qmm_paged_append_dev(const qmm_paged_kv* kv, const float* qkv_dev, s
             (q_norm_dev == nullptr) != (k_norm_dev == nullptr))
             return fail(QMM_ERR_INVALID_INPUT, "null pointer");
         const size_t row = ((size_t)n_heads + 2 * (size_t)a.kv.nkv) * a.kv.hd;
-        // one grid row holds every head vector, at least eight to a CTA
-        if (ld_qkv < row || ctx <= 0 || tokens > (size_t)INT32_MAX ||
-            tokens * (row / a.kv.hd) > (size_t)INT32_MAX * 8)
+        if (ld_qkv < row || ctx <= 0 || tokens > (size_t)INT32_MAX)
             return fail(QMM_ERR_SHAPE_MISMATCH, "row stride, context or token count out of range");
         if (!aligned16(qkv_dev) || ld_qkv % 4 || !aligned16(cos_dev) || !aligned16(sin_dev) || !aligned16(q_out_dev) ||
             !aligned16(q_norm_dev) || !aligned16(k_norm_dev))

@@ -28,93 +28,87 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
-// One group of G lanes (head_dim / 8 of them active) per head vector: a lane
-// holds elements [4 l, 4 l + 4) of each half, whole pairs in either order.
-// G: 8, 16 or 32.
+// A group of G lanes (head_dim / 8 of them active; G is 8, 16 or 32) per head
+// vector, CTAs of neighbouring heads of a token; a lane holds elements [4 l, 4 l + 4)
+// of each half, whole pairs in either order. Bound by HBM for long prompts as long
+// as a vector takes few instructions and registers (all of an SM's threads keep
+// their 32 bytes on the way): exact root and divide, 64-bit index arithmetic and
+// one vector per group 125 us for 8192 tokens, 64/8 heads of 128, bf16; four
+// vectors a group 134 us; persistent groups with two tokens on the way 127 us, bound
+// by instructions; this 102 us (6.26 TB/s).
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a, int G) {
-    const int lane = threadIdx.x & (G - 1);
-    const int hd = a.kv.hd, half = hd / 2;
-    const int heads = a.nq + 2 * a.kv.nkv;
-    const int64_t vec = (int64_t)blockIdx.x * (kAppendThreads / G) + threadIdx.x / G;
-    const int64_t token = vec / heads;
-    const int head = (int)(vec - token * heads);
-    const bool live = token < a.tokens && lane * 8 < hd;
-    float4 x = make_float4(0, 0, 0, 0), y = x;
-    int pos = -1;
-    if (live) {
-        const float* src = a.qkv + token * a.ld + (int64_t)head * hd;
-        x = *reinterpret_cast<const float4*>(src + 4 * lane);
-        y = *reinterpret_cast<const float4*>(src + half + 4 * lane);
-        pos = a.positions[token];
-    }
+__global__ void __launch_bounds__(kAppendThreads, 8) paged_append_kernel(const AppendArgs a, int G) {
+    const int lane4 = 4 * (threadIdx.x & (G - 1));
+    const int hd = a.kv.hd, half = hd >> 1;
+    const int token = blockIdx.x, head = blockIdx.y * (kAppendThreads / G) + threadIdx.x / G;
     const bool is_q = head < a.nq, is_v = head >= a.nq + a.kv.nkv;
-    const float* w = is_v ? nullptr : (is_q ? a.q_norm : a.k_norm);
-    // every lane of the warp takes part in the shuffles
-    float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + (y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
-    for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live) return;
-    const bool placed = pos >= 0 && pos < a.ctx;  // a rotation exists for the position
-    if (w) {
-        const float inv = 1.0f / sqrtf(ss / (float)hd + a.eps);
-        const float4 w0 = *reinterpret_cast<const float4*>(w + 4 * lane);
-        const float4 w1 = *reinterpret_cast<const float4*>(w + half + 4 * lane);
-        x.x = x.x * inv * (w0.x + a.offset);
-        x.y = x.y * inv * (w0.y + a.offset);
-        x.z = x.z * inv * (w0.z + a.offset);
-        x.w = x.w * inv * (w0.w + a.offset);
-        y.x = y.x * inv * (w1.x + a.offset);
-        y.y = y.y * inv * (w1.y + a.offset);
-        y.z = y.z * inv * (w1.z + a.offset);
-        y.w = y.w * inv * (w1.w + a.offset);
+    const bool live = lane4 < half && head < a.nq + 2 * a.kv.nkv;
+    float4 x = make_float4(0, 0, 0, 0), y = x;
+    if (live) {
+        const float* src = a.qkv + token * a.ld + (head * hd + lane4);
+        x = __ldcs(reinterpret_cast<const float4*>(src));
+        y = __ldcs(reinterpret_cast<const float4*>(src + half));
     }
+    const int pos = a.positions[token];
+    const bool placed = pos >= 0 && pos < a.ctx;  // a rotation exists for the position
+    if (a.q_norm) {                                // every lane of the warp takes part in the shuffles
+        float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + (y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
+        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (live && !is_v) {
+            const float* w = (is_q ? a.q_norm : a.k_norm) + lane4;
+            const float inv = rsqrtf(ss * (1.0f / (float)hd) + a.eps);  // to 2 ulp
+            const float4 w0 = *reinterpret_cast<const float4*>(w);
+            const float4 w1 = *reinterpret_cast<const float4*>(w + half);
+            x = make_float4(x.x * inv * (w0.x + a.offset), x.y * inv * (w0.y + a.offset),
+                            x.z * inv * (w0.z + a.offset), x.w * inv * (w0.w + a.offset));
+            y = make_float4(y.x * inv * (w1.x + a.offset), y.y * inv * (w1.y + a.offset),
+                            y.z * inv * (w1.z + a.offset), y.w * inv * (w1.w + a.offset));
+        }
+    }
+    if (!live) return;
     if (!is_v && placed) {
         const float* ct = a.cos_t + (int64_t)pos * half;
-        const float* sn = a.sin_t + (int64_t)pos * half;
-        const float4 p = x, r = y;
-        if constexpr (kInterleaved) {  // pairs 2 l, 2 l + 1 of the first half, and of the second
-            const float2 c0 = *reinterpret_cast<const float2*>(ct + 2 * lane);
-            const float2 s0 = *reinterpret_cast<const float2*>(sn + 2 * lane);
-            const float2 c1 = *reinterpret_cast<const float2*>(ct + half / 2 + 2 * lane);
-            const float2 s1 = *reinterpret_cast<const float2*>(sn + half / 2 + 2 * lane);
-            x = make_float4(p.x * c0.x - p.y * s0.x, p.x * s0.x + p.y * c0.x, p.z * c0.y - p.w * s0.y,
-                            p.z * s0.y + p.w * c0.y);
-            y = make_float4(r.x * c1.x - r.y * s1.x, r.x * s1.x + r.y * c1.x, r.z * c1.y - r.w * s1.y,
-                            r.z * s1.y + r.w * c1.y);
+        const float* st = a.sin_t + (int64_t)pos * half;
+        const float4 u = x, z = y;
+        if constexpr (kInterleaved) {  // pairs of the first half, then of the second
+            const int l = lane4 >> 1;
+            const float2 c0 = *reinterpret_cast<const float2*>(ct + l), s0 = *reinterpret_cast<const float2*>(st + l);
+            x = make_float4(u.x * c0.x - u.y * s0.x, u.x * s0.x + u.y * c0.x, u.z * c0.y - u.w * s0.y,
+                            u.z * s0.y + u.w * c0.y);
+            const float2 c1 = *reinterpret_cast<const float2*>(ct + (half >> 1) + l);
+            const float2 s1 = *reinterpret_cast<const float2*>(st + (half >> 1) + l);
+            y = make_float4(z.x * c1.x - z.y * s1.x, z.x * s1.x + z.y * c1.x, z.z * c1.y - z.w * s1.y,
+                            z.z * s1.y + z.w * c1.y);
         } else {
-            const float4 c = *reinterpret_cast<const float4*>(ct + 4 * lane);
-            const float4 s = *reinterpret_cast<const float4*>(sn + 4 * lane);
-            x = make_float4(p.x * c.x - r.x * s.x, p.y * c.y - r.y * s.y, p.z * c.z - r.z * s.z,
-                            p.w * c.w - r.w * s.w);
-            y = make_float4(p.x * s.x + r.x * c.x, p.y * s.y + r.y * c.y, p.z * s.z + r.z * c.z,
-                            p.w * s.w + r.w * c.w);
+            const float4 c = *reinterpret_cast<const float4*>(ct + lane4);
+            const float4 s = *reinterpret_cast<const float4*>(st + lane4);
+            x = make_float4(u.x * c.x - z.x * s.x, u.y * c.y - z.y * s.y, u.z * c.z - z.z * s.z,
+                            u.w * c.w - z.w * s.w);
+            y = make_float4(u.x * s.x + z.x * c.x, u.y * s.y + z.y * c.y, u.z * s.z + z.z * c.z,
+                            u.w * s.w + z.w * c.w);
         }
     }
     if (is_q) {
         if (!placed) x = y = make_float4(0, 0, 0, 0);
-        float* dst = a.q_out + (token * a.nq + head) * hd;
-        *reinterpret_cast<float4*>(dst + 4 * lane) = x;
-        *reinterpret_cast<float4*>(dst + half + 4 * lane) = y;
+        float* dst = a.q_out + ((int64_t)token * a.nq + head) * hd + lane4;
+        store4(dst, x);
+        store4(dst + half, y);
         return;
     }
-    if (!placed) return;
-    const int seq = a.seqs ? a.seqs[token] : (int)token;
-    const int slot = a.slots[token];
-    if (seq < 0 || seq >= a.kv.n_seqs || slot < 0 || slot >= a.kv.capacity()) return;
+    const int slot = a.slots[token], seq = a.seqs ? a.seqs[token] : token;
+    if (!placed || seq < 0 || seq >= a.kv.n_seqs || slot < 0 || slot >= a.kv.capacity()) return;
     const int64_t row = a.kv.row(seq, head - a.nq - (is_v ? a.kv.nkv : 0), slot);
     if (row < 0) return;
-    T* dst = static_cast<T*>(is_v ? a.kv.v : a.kv.k) + row;
-    store4(dst + 4 * lane, x);
-    store4(dst + half + 4 * lane, y);
+    T* dst = static_cast<T*>(is_v ? a.kv.v : a.kv.k) + row + lane4;
+    store4(dst, x);
+    store4(dst + half, y);
 }
 
 template <typename T>
 cudaError_t launch_append(const AppendArgs& a, bool interleaved, cudaStream_t st) {
     const int lanes = a.kv.hd / 8;
-    const int G = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32);
-    const int64_t vecs = (int64_t)a.tokens * (a.nq + 2 * a.kv.nkv);
-    const int64_t per = kAppendThreads / G;
-    const unsigned grid = (unsigned)((vecs + per - 1) / per);
+    const int G = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32), groups = kAppendThreads / G;
+    const dim3 grid(a.tokens, (a.nq + 2 * a.kv.nkv + groups - 1) / groups);
     if (interleaved) paged_append_kernel<T, true><<<grid, kAppendThreads, 0, st>>>(a, G);
     else paged_append_kernel<T, false><<<grid, kAppendThreads, 0, st>>>(a, G);
     note_launch();
