@@ -187,8 +187,6 @@ class Gemma3Decoder:
         self.rope = {t: (vec(c), vec(s)) for t, (c, s) in tabs.items()}
         B = batch
         z = lambda *shape: torch.zeros(*shape, dtype=torch.float32, device=dev)  # noqa: E731
-        self.k_cache = z(cfg.n_layers, B, nkv, cfg.ctx, hd)
-        self.v_cache = z(cfg.n_layers, B, nkv, cfg.ctx, hd)
         self.tokens = torch.zeros(B, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
         self.x, self.h, self.o = z(B, H), z(B, H), z(B, H)
@@ -197,19 +195,50 @@ class Gemma3Decoder:
         self.qkv, self.q, self.attn = z(B, nqkv), z(B, nq * hd), z(B, nq * hd)
         self.ff = z(B, Fl)
         self.logits = z(B, cfg.vocab)
-        self.part = z(int(self.lib.qmm_attention_partial_floats(B, nq, hd, cfg.ctx)))
         self.inv_scale = float(np.float32(1.0) / np.float32(math.sqrt(cfg.query_pre_attn_scalar)))
         self.stream = torch.cuda.Stream(dev)
         self.graph = None
+        self._alloc_cache()
         need = max(self.lib.qmm_workspace_size(dt, 0, B, n, k) for dt, n, k in
                    [(Q4_0, nqkv, kh), (Q4_0, H, nq * hd), (Q4_0, 2 * Fl, kh), (Q4_0, H, Fl),
                     (Q8_0, Vl, klm)])
         _lib.check(self.lib.qmm_reserve_workspace(device, ctypes.c_void_p(self.stream.cuda_stream), need + (1 << 20)))
 
+    def _alloc_cache(self) -> None:
+        cfg, B = self.cfg, self.batch
+        nq, nkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        z = lambda *shape: torch.zeros(*shape, dtype=torch.float32, device=self.dev)  # noqa: E731
+        self.k_cache = z(cfg.n_layers, B, nkv, cfg.ctx, hd)
+        self.v_cache = z(cfg.n_layers, B, nkv, cfg.ctx, hd)
+        self.part = z(int(self.lib.qmm_attention_partial_floats(B, nq, hd, cfg.ctx)))
+
     # ---- one step, issued on self.stream ---------------------------------------------
-    def _launch(self, advance: bool):
+    def _attention(self, li: int, lw: dict, cos: torch.Tensor, sin: torch.Tensor) -> None:
+        """Layer li's attention: self.qkv to self.attn, and k, v into its cache."""
         cfg, L, B = self.cfg, self.lib, self.batch
-        H, nq, nkv, hd = cfg.hidden, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        nq, nkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        sp = ctypes.c_void_p(self.stream.cuda_stream)
+        P = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+        ck = _lib.check
+        if self.fused_attention:
+            ck(L.qmm_attention_decode_fused_dev(P(self.qkv), B, nq, nkv, hd, P(lw["q_norm"]), P(lw["k_norm"]),
+                                                cfg.offset, cfg.eps, P(cos), P(sin), P(self.pos), cfg.ctx,
+                                                P(self.k_cache[li]), P(self.v_cache[li]), self.inv_scale,
+                                                P(self.part), P(self.attn), sp))
+        else:
+            ck(L.qmm_qk_rope_cache_dev(P(self.qkv), B, nq, nkv, hd, P(lw["q_norm"]), P(lw["k_norm"]), cfg.offset,
+                                       cfg.eps, P(cos), P(sin), P(self.pos), cfg.ctx, P(self.q),
+                                       P(self.k_cache[li]), P(self.v_cache[li]), sp))
+            ck(L.qmm_attention_decode_dev(P(self.q), P(self.k_cache[li]), P(self.v_cache[li]), B, nq, nkv, hd,
+                                          P(self.pos), cfg.ctx, self.inv_scale, P(self.part), P(self.attn), sp))
+
+    def _advance(self) -> None:
+        """Moves the step's position on."""
+        _lib.check(self.lib.qmm_add_int_dev(ctypes.c_void_p(self.pos.data_ptr()), 1,
+                                            ctypes.c_void_p(self.stream.cuda_stream)))
+
+    def _launch(self, advance: bool):
+        cfg, L, B, H = self.cfg, self.lib, self.batch, self.cfg.hidden
         sp = ctypes.c_void_p(self.stream.cuda_stream)
         P = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
         ck = _lib.check
@@ -221,17 +250,7 @@ class Gemma3Decoder:
             theta = cfg.rope_global if (li + 1) % cfg.pattern == 0 else cfg.rope_local
             cos, sin = self.rope[theta]
             ck(L.qmm_linear_forward(lw["qkv"].handle, P(self.hp), B, P(self.qkv), 0, sp))
-            if self.fused_attention:
-                ck(L.qmm_attention_decode_fused_dev(P(self.qkv), B, nq, nkv, hd, P(lw["q_norm"]), P(lw["k_norm"]),
-                                                    cfg.offset, cfg.eps, P(cos), P(sin), P(self.pos), cfg.ctx,
-                                                    P(self.k_cache[li]), P(self.v_cache[li]), self.inv_scale,
-                                                    P(self.part), P(self.attn), sp))
-            else:
-                ck(L.qmm_qk_rope_cache_dev(P(self.qkv), B, nq, nkv, hd, P(lw["q_norm"]), P(lw["k_norm"]), cfg.offset,
-                                           cfg.eps, P(cos), P(sin), P(self.pos), cfg.ctx, P(self.q),
-                                           P(self.k_cache[li]), P(self.v_cache[li]), sp))
-                ck(L.qmm_attention_decode_dev(P(self.q), P(self.k_cache[li]), P(self.v_cache[li]), B, nq, nkv, hd,
-                                              P(self.pos), cfg.ctx, self.inv_scale, P(self.part), P(self.attn), sp))
+            self._attention(li, lw, cos, sin)
             ck(L.qmm_linear_forward(lw["o"].handle, P(self.attn), B, P(self.o), 0, sp))
             ck(L.qmm_residual_rmsnorm_dev(P(self.x), P(self.o), P(lw["post_attn_norm"]), P(lw["ffn_norm"]),
                                           cfg.offset, cfg.eps, B, H, P(self.hp), self.kh, sp))
@@ -251,7 +270,7 @@ class Gemma3Decoder:
         else:
             ck(L.qmm_linear_forward(self.lm_head.handle, P(self.hl), B, P(self.logits), 0, sp))
         if advance:
-            ck(L.qmm_add_int_dev(P(self.pos), 1, sp))
+            self._advance()
 
     def set_position(self, pos: int) -> None:
         if not 0 <= pos < self.cfg.ctx:
