@@ -26,7 +26,6 @@ namespace qmm {
 
 namespace {
 
-constexpr int kHeadTile = 8;  // query heads of one kv head that share a pass over its K and V
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- matrix instructions ----------------------------------------------------------
@@ -149,8 +148,8 @@ __device__ __forceinline__ Slots slots_of(const AttendArgs& a, int b) {
 // that is not the whole leaves (acc, m, l) behind: in the CTA's slot 0 if earlier
 // CTAs hold the beginning, in slot 1 if not.
 struct Scratch {
-    float2* ml;      // [grid][2][kHeadTile]: reference and sum of a piece (see kSlack)
-    float* acc;      // [grid][2][kHeadTile][hd]
+    float2* ml;      // [grid][2][kHeads]: reference and sum of a piece (see kSlack)
+    float* acc;      // [grid][2][kHeads][hd]
     float2* whole;   // [n_seqs][nq], with weights: the same of undivided head tiles
     float* scores;   // [n_seqs][nq][capacity], with weights: scores in units of log 2
     int head_tiles;  // per kv head
@@ -203,14 +202,18 @@ __device__ __forceinline__ Place place_of(const AttendArgs& a, const Scratch& sc
     return Place{warp_sum64(before), share_of<S>(warp_sum64(total), sc.grid), slots_of<S::kSlots>(a, b).tiles};
 }
 
+// kSets sets of 8 query heads of a kv head share a pass over its K and V: two
+// where there are more than 8 (16 heads on one: a pass for each eight 73 us for
+// 200 MB of K and V, one for both SETSUS).
 // kTile slots are the K of one instruction's P; a step takes kTiles of them. A
 // warp's ring holds three units of a step's K or V rows: one in use, two on
 // their way (16 warps per SM with 4 KB units: 128 KB in flight, above the 44 KB
 // that 6.5 TB/s and 1 us need).
-template <typename T, int HD>
+template <typename T, int HD, int SETS>
 struct Shape {
+    static constexpr int kHeads = 8 * SETS;
     static constexpr int kTile = sizeof(T) == 4 ? 8 : 16;
-    static constexpr int kTiles = HD <= 64 ? 2 : 1;
+    static constexpr int kTiles = HD <= 64 || (HD <= 128 && SETS > 1) ? 2 : 1;
     static constexpr int kSlots = kTile * kTiles;
     static constexpr int kRow = HD * (int)sizeof(T);             // bytes
     static constexpr int kChunks = kRow / 64;                    // 16-byte units of a K row per lane
@@ -218,14 +221,15 @@ struct Shape {
     static constexpr int kVRows = kTile / 4;                     // V rows of a tile per lane
     static constexpr int kUnit = kSlots * HD * (int)sizeof(T);
     static constexpr int kUnits = 3;
-    static constexpr int kWarps = HD <= 128 ? 8 : (HD <= 192 ? 5 : 4);
-    static constexpr int kCtas = 2;                              // per SM
+    static constexpr int kWarps = HD <= 64 || (HD <= 128 && SETS == 1) ? 8 : (HD == 192 && SETS == 1 ? 5 : 4);
+    static constexpr int kQBytes = kChunks * 2 * 32 * 16;        // of a set
+    static constexpr bool kQRegs = SETS == 1 && kChunks <= (kWarps == 8 ? 4 : 8);  // Q in registers
     static constexpr int kSetup = 163840 / (2 * kUnit);          // a piece's fixed cost in steps: 6 us measured
-    static constexpr int kQBytes = kChunks * 2 * 32 * 16;
-    static constexpr bool kQRegs = kChunks <= (kWarps == 8 ? 4 : 8);  // Q in registers
     static constexpr int kAccRow = HD + 4;                       // floats; spreads the rows over the banks
-    static constexpr size_t kSmem = (size_t)kWarps * kUnits * kUnit + kQBytes + kWarps * kHeadTile * 8 + kHeadTile * 4;
-    static_assert(kHeadTile * kAccRow * 4 <= kUnits * kUnit, "a warp's result fits in its ring");
+    static constexpr size_t kSmem =
+        (size_t)kWarps * kUnits * kUnit + SETS * kQBytes + kWarps * kHeads * 8 + kHeads * 4;
+    static constexpr int kCtas = 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;  // per SM
+    static_assert(kHeads * kAccRow * 4 <= kUnits * kUnit, "a warp's result fits in its ring");
 };
 
 // Weights are relative to 2^m with m at most kSlack below the largest score so
@@ -254,10 +258,10 @@ constexpr float kSlack = std::is_same_v<T, __half> ? 1.0f : 8.0f;
 // with the parts as rows took as many, but twice the accumulators: 8 warps per SM
 // for 16.) K and V in f32
 // are split too.
-template <typename T, int HD>
-__global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas)
+template <typename T, int HD, int SETS>
+__global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, SETS>::kCtas)
     attend_kernel(const AttendArgs a, const Scratch sc) {
-    using S = Shape<T, HD>;
+    using S = Shape<T, HD, SETS>;
     constexpr int W = S::kWarps, kSlots = S::kSlots, kTiles = S::kTiles, kTile = S::kTile;
     constexpr int kElems = 16 / (int)sizeof(T);  // of a 16-byte unit
     extern __shared__ __align__(16) uint8_t smem[];
@@ -276,8 +280,8 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
     const int k_half[2] = {(g & 1) * 64, 64 - (g & 1) * 64};
     const uint8_t* v_src = ring + 2 * t * S::kRow + (g ^ (2 * t)) * 16;
     uint8_t* qs = smem + W * S::kUnits * S::kUnit;
-    float2* ml_s = reinterpret_cast<float2*>(qs + S::kQBytes);        // [W][kHeadTile]
-    float* unit_s = reinterpret_cast<float*>(ml_s + W * kHeadTile);   // [kHeadTile]
+    float2* ml_s = reinterpret_cast<float2*>(qs + SETS * S::kQBytes);  // [W][kHeads]
+    float* unit_s = reinterpret_cast<float*>(ml_s + W * S::kHeads);    // [kHeads]
     const int group = a.nq / a.kv.nkv;
     const int heads = a.kv.nkv * sc.head_tiles;  // head tiles of a sequence
 
@@ -313,8 +317,8 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
     while (base < end) {
         const int tile = (int)max(begin - base, (int64_t)0);
         const int count = (int)min(end - base, (int64_t)s.tiles) - tile;  // at least 1: see the step to the next
-        const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * kHeadTile;
-        const int nh = min(kHeadTile, group - q0);
+        const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * S::kHeads;
+        const int nh = min(S::kHeads, group - q0);
         const int head0 = kvh * group + q0;
         const int* table = a.kv.table + b * a.kv.table_stride;
         const int mask = (1 << a.kv.page_shift) - 1;
@@ -368,7 +372,7 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
         pages = pages_of(1);
 
         // Q of the head tile in the order of operand A, its power of two taken out
-        for (int j = warp; j < kHeadTile; j += W) {
+        for (int j = warp; j < S::kHeads; j += W) {
             const float* q = a.q + b * a.ldq + (int64_t)(head0 + j) * HD;
             float x[HD / 32], top = 0.0f;
 #pragma unroll
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
                 const int step = (c >> 2) * 2 + r / (kElems / 2), p = r % (kElems / 2);
                 T hi, lo;
                 split<T>(x[i] * down, &hi, &lo);
-                T* dst = reinterpret_cast<T*>(qs + (step * 32 + j * 4 + (c & 3)) * 16);
+                T* dst = reinterpret_cast<T*>(qs + (j >> 3) * S::kQBytes + (step * 32 + (j & 7) * 4 + (c & 3)) * 16);
                 if constexpr (sizeof(T) == 4) {
                     dst[2 * p] = hi;
                     dst[2 * p + 1] = lo;
@@ -398,19 +402,26 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
             }
         }
         __syncthreads();
-        const float unit = unit_s[g];
         const uint8_t* qs_l = qs + lane * 16;
         uint4 qr[S::kQRegs ? 2 * S::kChunks : 1];
         if constexpr (S::kQRegs) {
 #pragma unroll
             for (int j = 0; j < 2 * S::kChunks; ++j) qr[j] = lds16(qs_l + j * 512);
         }
-        float* srow = sc.scores && g < nh ? sc.scores + ((int64_t)b * a.nq + head0 + g) * a.kv.capacity() : nullptr;
-
-        float m = -INFINITY, l = 0.0f, lc = 0.0f;
-        float acc[HD / 16][4];  // [two columns]: head 2 t, head 2 t + 1 at the first; the same at the second
+        float unit[SETS], m[SETS], l[SETS], lc[SETS];
+        float* srow[SETS];
+        float acc[SETS][HD / 16][4];  // [two columns]: head 2 t, head 2 t + 1 at the first; the same at the second
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+        for (int q = 0; q < SETS; ++q) {
+            unit[q] = unit_s[8 * q + g];
+            srow[q] = sc.scores && 8 * q + g < nh
+                          ? sc.scores + ((int64_t)b * a.nq + head0 + 8 * q + g) * a.kv.capacity()
+                          : nullptr;
+            m[q] = -INFINITY;
+            l[q] = lc[q] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) acc[q][i][0] = acc[q][i][1] = acc[q][i][2] = acc[q][i][3] = 0.0f;
+        }
 
         int at = 0;  // the unit of K of step i; V follows
         for (int i = 0; i < my; ++i) {
@@ -420,37 +431,49 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
             issue(i + 1, pages, a.kv.k, spare, false);
             const Pages after = pages_of(i + 2);
             const uint8_t* src = k_src + at * S::kUnit;
-            // scores: two chains of products per 8 slots
+            // scores: two chains of products per 8 slots and set
             constexpr int kX = kSlots / 4;
-            float x[kX];
+            float x[SETS][kX];
 #pragma unroll
             for (int r = 0; r < kSlots / 8; ++r) {
-                float c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
+                float c0[SETS][4] = {}, c1[SETS][4] = {};
 #pragma unroll
                 for (int j = 0; j < S::kChunks; ++j) {
                     const uint4 k = lds16(src + 8 * r * S::kRow + (j >> 1) * 128 + k_half[j & 1]);
-                    uint4 qa, qb;
-                    if constexpr (S::kQRegs) qa = qr[2 * j], qb = qr[2 * j + 1];
-                    else qa = lds16(qs_l + (2 * j) * 512), qb = lds16(qs_l + (2 * j + 1) * 512);
+                    float hi[4], lo[4];
                     if constexpr (sizeof(T) == 4) {
-                        float hi[4], lo[4];
                         split<T>(__uint_as_float(k.x), &hi[0], &lo[0]);
                         split<T>(__uint_as_float(k.y), &hi[1], &lo[1]);
                         split<T>(__uint_as_float(k.z), &hi[2], &lo[2]);
                         split<T>(__uint_as_float(k.w), &hi[3], &lo[3]);
-                        mma<T>(c0, qa, __float_as_uint(hi[0]), __float_as_uint(hi[1]));
-                        mma<T>(c1, qb, __float_as_uint(hi[2]), __float_as_uint(hi[3]));
-                        mma<T>(c0, qa, __float_as_uint(lo[0]), __float_as_uint(lo[1]));
-                        mma<T>(c1, qb, __float_as_uint(lo[2]), __float_as_uint(lo[3]));
-                    } else {
-                        mma<T>(c0, qa, k.x, k.y);
-                        mma<T>(c1, qb, k.z, k.w);
+                    }
+#pragma unroll
+                    for (int q = 0; q < SETS; ++q) {
+                        uint4 qa, qb;
+                        if constexpr (S::kQRegs) {
+                            qa = qr[2 * j], qb = qr[2 * j + 1];
+                        } else {
+                            qa = lds16(qs_l + q * S::kQBytes + (2 * j) * 512);
+                            qb = lds16(qs_l + q * S::kQBytes + (2 * j + 1) * 512);
+                        }
+                        if constexpr (sizeof(T) == 4) {
+                            mma<T>(c0[q], qa, __float_as_uint(hi[0]), __float_as_uint(hi[1]));
+                            mma<T>(c1[q], qb, __float_as_uint(hi[2]), __float_as_uint(hi[3]));
+                            mma<T>(c0[q], qa, __float_as_uint(lo[0]), __float_as_uint(lo[1]));
+                            mma<T>(c1[q], qb, __float_as_uint(lo[2]), __float_as_uint(lo[3]));
+                        } else {
+                            mma<T>(c0[q], qa, k.x, k.y);
+                            mma<T>(c1[q], qb, k.z, k.w);
+                        }
                     }
                 }
-                x[2 * r] = ((c0[0] + c1[0]) + (c0[2] + c1[2])) * unit;
-                x[2 * r + 1] = ((c0[1] + c1[1]) + (c0[3] + c1[3])) * unit;
+#pragma unroll
+                for (int q = 0; q < SETS; ++q) {
+                    x[q][2 * r] = ((c0[q][0] + c1[q][0]) + (c0[q][2] + c1[q][2])) * unit[q];
+                    x[q][2 * r + 1] = ((c0[q][1] + c1[q][1]) + (c0[q][3] + c1[q][3])) * unit[q];
+                }
             }
-            // lane (g, t) has the scores of head g at slots 2 t, 2 t + 1 of every eight
+            // lane (g, t) has the scores of heads g, g + 8 at slots 2 t, 2 t + 1 of every eight
             const int slot0 = my_slot0 + i * (W * kSlots);
             bool whole = slot0 >= s.first && slot0 + kSlots <= s.n;
 #pragma unroll
@@ -460,58 +483,63 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
                 for (int r = 0; r < kX; ++r) {
                     const int slot = slot0 + 2 * t + (r & 1) + 8 * (r >> 1);
                     const int page = seen.p[r * 4 / kTile];
-                    if (page < 0 || page >= a.kv.n_pages || slot < s.first || slot >= s.n) x[r] = -INFINITY;
+                    if (page < 0 || page >= a.kv.n_pages || slot < s.first || slot >= s.n)
+#pragma unroll
+                        for (int q = 0; q < SETS; ++q) x[q][r] = -INFINITY;
                 }
             }
-            if (srow) {
+            uint4 p[SETS][kTiles];  // operand B: high parts x, y, low parts z, w
+#pragma unroll
+            for (int q = 0; q < SETS; ++q) {
+                if (srow[q]) {
+#pragma unroll
+                    for (int r = 0; r < kX; ++r) {
+                        const int slot = slot0 + 2 * t + (r & 1) + 8 * (r >> 1);
+                        if (slot >= s.first && slot < s.n) srow[q][slot] = x[q][r];
+                    }
+                }
+                float top = x[q][0];
+#pragma unroll
+                for (int r = 1; r < kX; ++r) top = fmaxf(top, x[q][r]);
+                top = quad_max(top);
+                if (__any_sync(0xffffffffu, top > m[q] + kSlack<T>)) {
+                    const float up = fmaxf(m[q], top), f = up == -INFINITY ? 1.0f : ex2(m[q] - up);
+                    const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+                    for (int j = 0; j < HD / 16; ++j) {
+                        acc[q][j][0] *= f0;
+                        acc[q][j][1] *= f1;
+                        acc[q][j][2] *= f0;
+                        acc[q][j][3] *= f1;
+                    }
+                    l[q] *= f;
+                    lc[q] *= f;
+                    m[q] = up;
+                }
+                const float zero = m[q] == -INFINITY ? 0.0f : m[q] - kWeightBias<T>;
+                float sum = 0.0f;
 #pragma unroll
                 for (int r = 0; r < kX; ++r) {
-                    const int slot = slot0 + 2 * t + (r & 1) + 8 * (r >> 1);
-                    if (slot >= s.first && slot < s.n) srow[slot] = x[r];
+                    x[q][r] = ex2(x[q][r] - zero);
+                    sum += x[q][r];
                 }
-            }
-            float top = x[0];
+                // the rounding error of the sum is carried along: many small weights beside a large one count
+                lc[q] += sum;
+                const float l2 = l[q] + lc[q];
+                lc[q] -= l2 - l[q];
+                l[q] = l2;
 #pragma unroll
-            for (int r = 1; r < kX; ++r) top = fmaxf(top, x[r]);
-            top = quad_max(top);
-            if (__any_sync(0xffffffffu, top > m + kSlack<T>)) {
-                const float up = fmaxf(m, top), f = up == -INFINITY ? 1.0f : ex2(m - up);
-                const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j) {
-                    acc[j][0] *= f0;
-                    acc[j][1] *= f1;
-                    acc[j][2] *= f0;
-                    acc[j][3] *= f1;
-                }
-                l *= f;
-                lc *= f;
-                m = up;
-            }
-            const float zero = m == -INFINITY ? 0.0f : m - kWeightBias<T>;
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < kX; ++r) {
-                x[r] = ex2(x[r] - zero);
-                sum += x[r];
-            }
-            // the rounding error of the sum is carried along: many small weights beside a large one count
-            lc += sum;
-            const float l2 = l + lc;
-            lc -= l2 - l;
-            l = l2;
-            uint4 p[kTiles];  // operand B: high parts x, y, low parts z, w
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u) {
-                if constexpr (sizeof(T) == 4) {
-                    float hi[2], lo[2];
-                    split<T>(x[2 * u], &hi[0], &lo[0]);
-                    split<T>(x[2 * u + 1], &hi[1], &lo[1]);
-                    p[u] = make_uint4(__float_as_uint(hi[0]), __float_as_uint(hi[1]), __float_as_uint(lo[0]),
-                                      __float_as_uint(lo[1]));
-                } else {
-                    split2<T>(x[4 * u], x[4 * u + 1], &p[u].x, &p[u].z);
-                    split2<T>(x[4 * u + 2], x[4 * u + 3], &p[u].y, &p[u].w);
+                for (int u = 0; u < kTiles; ++u) {
+                    if constexpr (sizeof(T) == 4) {
+                        float hi[2], lo[2];
+                        split<T>(x[q][2 * u], &hi[0], &lo[0]);
+                        split<T>(x[q][2 * u + 1], &hi[1], &lo[1]);
+                        p[q][u] = make_uint4(__float_as_uint(hi[0]), __float_as_uint(hi[1]), __float_as_uint(lo[0]),
+                                             __float_as_uint(lo[1]));
+                    } else {
+                        split2<T>(x[q][4 * u], x[q][4 * u + 1], &p[q][u].x, &p[q][u].z);
+                        split2<T>(x[q][4 * u + 2], x[q][4 * u + 3], &p[q][u].y, &p[q][u].w);
+                    }
                 }
             }
             copy_wait<1>();
@@ -542,9 +570,12 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
                                                         __float_as_uint(hi[2]), __float_as_uint(hi[3]));
                             const uint4 vl = make_uint4(__float_as_uint(lo[0]), __float_as_uint(lo[1]),
                                                         __float_as_uint(lo[2]), __float_as_uint(lo[3]));
-                            mma<T>(acc[j * 2 + e], vh, p[u].x, p[u].y);
-                            mma<T>(acc[j * 2 + e], vl, p[u].x, p[u].y);
-                            mma<T>(acc[j * 2 + e], vh, p[u].z, p[u].w);
+#pragma unroll
+                            for (int q = 0; q < SETS; ++q) {
+                                mma<T>(acc[q][j * 2 + e], vh, p[q][u].x, p[q][u].y);
+                                mma<T>(acc[q][j * 2 + e], vl, p[q][u].x, p[q][u].y);
+                                mma<T>(acc[q][j * 2 + e], vh, p[q][u].z, p[q][u].w);
+                            }
                         }
                     } else {
                         const uint32_t v2[4] = {v[2].x, v[2].y, v[2].z, v[2].w};
@@ -555,8 +586,11 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
                                                         __byte_perm(v0[e], v1[e], 0x7632),
                                                         __byte_perm(v2[e], v3[e], 0x5410),
                                                         __byte_perm(v2[e], v3[e], 0x7632));
-                            mma<T>(acc[j * 4 + e], vv, p[u].x, p[u].y);
-                            mma<T>(acc[j * 4 + e], vv, p[u].z, p[u].w);
+#pragma unroll
+                            for (int q = 0; q < SETS; ++q) {
+                                mma<T>(acc[q][j * 4 + e], vv, p[q][u].x, p[q][u].y);
+                                mma<T>(acc[q][j * 4 + e], vv, p[q][u].z, p[q][u].w);
+                            }
                         }
                     }
                 }
@@ -564,20 +598,24 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
         }
         copy_wait<0>();
 
-        // the warps' results, each in its own ring: heads 2 t, 2 t + 1, the columns of the lane's V units
+        // the warps' results, each in its own ring: heads 2 t, 2 t + 1 of a set, the columns of the lane's V units
         float* mine_s = reinterpret_cast<float*>(ring);
 #pragma unroll
-        for (int j = 0; j < S::kLines; ++j)
+        for (int q = 0; q < SETS; ++q) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int j = 0; j < S::kLines; ++j)
 #pragma unroll
-                for (int e = 0; e < kElems; e += 4) {
-                    const int i = (j * kElems + e) / 2;
-                    *reinterpret_cast<float4*>(mine_s + (2 * t + half) * S::kAccRow + (j * 8 + g) * kElems + e) =
-                        make_float4(acc[i][half], acc[i][2 + half], acc[i + 1][half], acc[i + 1][2 + half]);
-                }
-        l = quad_sum(l + lc);
-        if (t == 0) ml_s[warp * kHeadTile + g] = make_float2(m, l);
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int e = 0; e < kElems; e += 4) {
+                        const int i = (j * kElems + e) / 2;
+                        *reinterpret_cast<float4*>(mine_s + (8 * q + 2 * t + half) * S::kAccRow + (j * 8 + g) * kElems +
+                                                   e) = make_float4(acc[q][i][half], acc[q][i][2 + half],
+                                                                    acc[q][i + 1][half], acc[q][i + 1][2 + half]);
+                    }
+            const float sum = quad_sum(l[q] + lc[q]);
+            if (t == 0) ml_s[warp * S::kHeads + 8 * q + g] = make_float2(m[q], sum);
+        }
         __syncthreads();
         const bool begins = tile == 0, ends = tile + count == s.tiles;
         const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
@@ -585,11 +623,11 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
             const int j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; ++w) M = fmaxf(M, ml_s[w * kHeadTile + j].x);
+            for (int w = 0; w < W; ++w) M = fmaxf(M, ml_s[w * S::kHeads + j].x);
             float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float2 ml = ml_s[w * kHeadTile + j];
+                const float2 ml = ml_s[w * S::kHeads + j];
                 const float f = piece_factor(ml.x, M);
                 L += ml.y * f;
                 const float4 p = *reinterpret_cast<const float4*>(
@@ -605,8 +643,8 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
                     make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
                 if (sc.whole && d == 0) sc.whole[(int64_t)b * a.nq + head0 + j] = make_float2(M, L);
             } else {
-                *reinterpret_cast<float4*>(sc.acc + ((int64_t)slot * kHeadTile + j) * HD + d) = o;
-                if (d == 0) sc.ml[slot * kHeadTile + j] = make_float2(M, L);
+                *reinterpret_cast<float4*>(sc.acc + ((int64_t)slot * S::kHeads + j) * HD + d) = o;
+                if (d == 0) sc.ml[slot * S::kHeads + j] = make_float2(M, L);
             }
         }
         base += s.tiles + S::kSetup;
@@ -622,14 +660,14 @@ __global__ void __launch_bounds__(Shape<T, HD>::kWarps * 32, Shape<T, HD>::kCtas
 
 // Joins the pieces of divided (sequence, head tile)s in the order of the CTAs
 // that left them, and writes the zeros of sequences without slots. A CTA takes
-// kHeads heads of a head tile: one (blockIdx.y-th) where there are few head tiles
-// with many pieces, all eight where there are many. A thread sums four columns
+// kHeads heads of a head tile: one where there are few head tiles with many
+// pieces, eight where there are many. A thread sums four columns
 // of a head over every kGroups-th piece.
 // It is on the way of every small call, so it is launched early (programmatic
 // dependent launch), finds the pieces from the lengths before it waits for
 // attend_kernel, and has one round of loads after it.
 // With weights, the CTAs from join_blocks on add the slots' weights.
-template <typename T, int HD, int kHeads>
+template <int HD, int kHeads>
 struct JoinShape {
     static constexpr int kCols = HD / 4;
     static constexpr int kThreads = kHeads * kCols < 256 ? 256 : kHeads * kCols;
@@ -640,9 +678,8 @@ struct JoinShape {
 
 // weights_out[b][kvh][t] = weights[b][kvh][t] + sum over the kv head's query
 // heads of e^(s_t - m) / sum e^(s - m), four slots a thread.
-template <typename T, int HD, int kThreads, int kHeadsAtOnce>
+template <typename T, typename S, int kThreads, int kHeadsAtOnce>
 __device__ __forceinline__ void add_weights(const AttendArgs& a, const Scratch& sc, int64_t block) {
-    using S = Shape<T, HD>;
     __shared__ float2 zero_inv[kHeadsAtOnce];  // what to subtract from a score, what to multiply its power with
     const int64_t cap = a.kv.capacity();
     const int64_t blocks = (cap / 4 + kThreads - 1) / kThreads;  // of a (sequence, kv head)
@@ -668,17 +705,17 @@ __device__ __forceinline__ void add_weights(const AttendArgs& a, const Scratch& 
         if (g0) __syncthreads();
         for (int i = warp; i < heads; i += kThreads / 32) {
             const int j = g0 + i;
-            const Pieces pc = place.pieces<S>(kvh * sc.head_tiles + j / kHeadTile);
+            const Pieces pc = place.pieces<S>(kvh * sc.head_tiles + j / S::kHeads);
             float M = -INFINITY, L = 0.0f;
             if (pc.count == 1) {
                 const float2 ml = sc.whole[head0 + j];
                 M = ml.x;
                 L = ml.y;
             } else {
-                for (int q = lane; q < pc.count; q += 32) M = fmaxf(M, sc.ml[pc.slot(q) * kHeadTile + j % kHeadTile].x);
+                for (int q = lane; q < pc.count; q += 32) M = fmaxf(M, sc.ml[pc.slot(q) * S::kHeads + j % S::kHeads].x);
                 M = warp_max(M);
                 for (int q = lane; q < pc.count; q += 32) {
-                    const float2 ml = sc.ml[pc.slot(q) * kHeadTile + j % kHeadTile];
+                    const float2 ml = sc.ml[pc.slot(q) * S::kHeads + j % S::kHeads];
                     L += ml.y * piece_factor(ml.x, M);
                 }
                 L = warp_sum(L);
@@ -709,25 +746,25 @@ __device__ __forceinline__ void add_weights(const AttendArgs& a, const Scratch& 
     *reinterpret_cast<float4*>(a.weights_out + at) = w;
 }
 
-template <typename T, int HD, int kHeads>
-__global__ void __launch_bounds__(JoinShape<T, HD, kHeads>::kThreads)
+template <typename T, int HD, int SETS, int kHeads>
+__global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
     join_kernel(const AttendArgs a, const Scratch sc, unsigned join_blocks) {
-    using S = Shape<T, HD>;
-    using J = JoinShape<T, HD, kHeads>;
+    using S = Shape<T, HD, SETS>;
+    using J = JoinShape<HD, kHeads>;
     constexpr int kCols = J::kCols, kGroups = J::kGroups, kWarps = J::kThreads / 32, kAhead = J::kAhead;
     extern __shared__ float factors[];  // [kHeads][grid]
     __shared__ float4 part[kGroups][kHeads][kCols];
     __shared__ float inv_s[kHeads];
     if (blockIdx.x >= join_blocks) {
-        if (blockIdx.y == 0) add_weights<T, HD, J::kThreads, J::kHeadsAtOnce>(a, sc, blockIdx.x - join_blocks);
+        if (blockIdx.y == 0) add_weights<T, S, J::kThreads, J::kHeadsAtOnce>(a, sc, blockIdx.x - join_blocks);
         else pdl_wait();
         return;
     }
     const int heads = a.kv.nkv * sc.head_tiles;
     const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
     const int group = a.nq / a.kv.nkv;
-    const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * kHeadTile;
-    const int j0 = blockIdx.y * kHeads, nh = min(kHeads, min(kHeadTile, group - q0) - j0);
+    const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * S::kHeads;
+    const int j0 = blockIdx.y * kHeads, nh = min(kHeads, min(S::kHeads, group - q0) - j0);
     const int64_t head0 = (int64_t)b * a.nq + kvh * group + q0 + j0;
     const int unit = threadIdx.x / kCols, col = threadIdx.x - unit * kCols;
     const int grp = unit / kHeads, j = unit - grp * kHeads;
@@ -743,7 +780,7 @@ __global__ void __launch_bounds__(JoinShape<T, HD, kHeads>::kThreads)
     if (pc.count == 1) return;  // written by its CTA
     const bool mine = grp < kGroups && j < nh;
     auto load = [&](int p) {
-        return reinterpret_cast<const float4*>(sc.acc + (pc.slot(p) * kHeadTile + j0 + j) * HD)[col];
+        return reinterpret_cast<const float4*>(sc.acc + (pc.slot(p) * S::kHeads + j0 + j) * HD)[col];
     };
     float4 ahead[kAhead];
 #pragma unroll
@@ -753,12 +790,12 @@ __global__ void __launch_bounds__(JoinShape<T, HD, kHeads>::kThreads)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = warp; i < nh; i += kWarps) {
         const float2* ml = sc.ml + j0 + i;
-        float2 first = lane < pc.count ? ml[pc.slot(lane) * kHeadTile] : make_float2(-INFINITY, 0.0f);
+        float2 first = lane < pc.count ? ml[pc.slot(lane) * S::kHeads] : make_float2(-INFINITY, 0.0f);
         float M = first.x, L = 0.0f;
-        for (int p = lane + 32; p < pc.count; p += 32) M = fmaxf(M, ml[pc.slot(p) * kHeadTile].x);
+        for (int p = lane + 32; p < pc.count; p += 32) M = fmaxf(M, ml[pc.slot(p) * S::kHeads].x);
         M = warp_max(M);
         for (int p = lane; p < pc.count; p += 32) {
-            const float2 v = p == lane ? first : ml[pc.slot(p) * kHeadTile];
+            const float2 v = p == lane ? first : ml[pc.slot(p) * S::kHeads];
             const float f = piece_factor(v.x, M);
             factors[i * sc.grid + p] = f;
             L += v.y * f;
@@ -797,7 +834,8 @@ __global__ void __launch_bounds__(JoinShape<T, HD, kHeads>::kThreads)
     *out = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-int head_tiles(const PagedKv& kv, int nq) { return (nq / kv.nkv + kHeadTile - 1) / kHeadTile; }
+// Query heads of a pass over K and V: one set of 8, or two.
+int pass_heads(const PagedKv& kv, int nq) { return nq / kv.nkv > 8 ? 16 : 8; }
 
 int sm_count() {
     int dev = 0, sms = 0;
@@ -818,9 +856,10 @@ size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Scra
         off += aligned(bytes);
         return p;
     };
-    sc->head_tiles = head_tiles(kv, nq);
-    sc->ml = static_cast<float2*>(take((size_t)grid * 2 * kHeadTile * sizeof(float2)));
-    sc->acc = static_cast<float*>(take((size_t)grid * 2 * kHeadTile * kv.hd * sizeof(float)));
+    const int heads = pass_heads(kv, nq);
+    sc->head_tiles = (nq / kv.nkv + heads - 1) / heads;
+    sc->ml = static_cast<float2*>(take((size_t)grid * 2 * heads * sizeof(float2)));
+    sc->acc = static_cast<float*>(take((size_t)grid * 2 * heads * kv.hd * sizeof(float)));
     sc->whole = nullptr;
     sc->scores = nullptr;
     if (weights) {
@@ -830,43 +869,48 @@ size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Scra
     return off;
 }
 
-template <typename T, int HD, int kHeads>
+template <typename T, int HD, int SETS, int kHeads>
 cudaError_t launch_join(AttendArgs a, Scratch sc, int grid_y, cudaStream_t st) {
-    using J = JoinShape<T, HD, kHeads>;
+    using J = JoinShape<HD, kHeads>;
     unsigned join_blocks = (unsigned)(a.kv.n_seqs * a.kv.nkv * sc.head_tiles);
     int64_t blocks = join_blocks;
     if (a.weights)
         blocks += (int64_t)a.kv.n_seqs * a.kv.nkv * ((a.kv.capacity() / 4 + J::kThreads - 1) / J::kThreads);
     if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
     void* args[] = {&a, &sc, &join_blocks};
-    return launch_pdl_kernel((const void*)join_kernel<T, HD, kHeads>, dim3((unsigned)blocks, grid_y),
+    return launch_pdl_kernel((const void*)join_kernel<T, HD, SETS, kHeads>, dim3((unsigned)blocks, grid_y),
                              dim3(J::kThreads), kHeads * sc.grid * sizeof(float), st, args);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int SETS>
 cudaError_t launch(const AttendArgs& a, Scratch sc, int sms, cudaStream_t st) {
-    using S = Shape<T, HD>;
-    cudaError_t e = ensure_dynamic_smem((const void*)attend_kernel<T, HD>, S::kSmem);
+    using S = Shape<T, HD, SETS>;
+    cudaError_t e = ensure_dynamic_smem((const void*)attend_kernel<T, HD, SETS>, S::kSmem);
     if (e != cudaSuccess) return e;
     sc.grid = sms * S::kCtas;
-    attend_kernel<T, HD><<<sc.grid, S::kWarps * 32, S::kSmem, st>>>(a, sc);
+    attend_kernel<T, HD, SETS><<<sc.grid, S::kWarps * 32, S::kSmem, st>>>(a, sc);
     note_launch();
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int tiles = a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
-    const int heads = a.nq / a.kv.nkv < kHeadTile ? a.nq / a.kv.nkv : kHeadTile;
+    const int heads = a.nq / a.kv.nkv < S::kHeads ? a.nq / a.kv.nkv : S::kHeads;
     // few head tiles: their heads side by side
-    if ((int64_t)tiles * heads <= 8 * sms) return launch_join<T, HD, 1>(a, sc, heads, st);
-    return launch_join<T, HD, kHeadTile>(a, sc, 1, st);
+    if ((int64_t)tiles * heads <= 8 * sms) return launch_join<T, HD, SETS, 1>(a, sc, heads, st);
+    return launch_join<T, HD, SETS, 8>(a, sc, SETS, st);
+}
+
+template <typename T, int HD>
+cudaError_t launch_sets(const AttendArgs& a, const Scratch& sc, int sms, cudaStream_t st) {
+    return pass_heads(a.kv, a.nq) == 8 ? launch<T, HD, 1>(a, sc, sms, st) : launch<T, HD, 2>(a, sc, sms, st);
 }
 
 template <typename T>
 cudaError_t launch_hd(const AttendArgs& a, const Scratch& sc, int sms, cudaStream_t st) {
     switch (a.kv.hd) {
-        case 64: return launch<T, 64>(a, sc, sms, st);
-        case 128: return launch<T, 128>(a, sc, sms, st);
-        case 192: return launch<T, 192>(a, sc, sms, st);
-        case 256: return launch<T, 256>(a, sc, sms, st);
+        case 64: return launch_sets<T, 64>(a, sc, sms, st);
+        case 128: return launch_sets<T, 128>(a, sc, sms, st);
+        case 192: return launch_sets<T, 192>(a, sc, sms, st);
+        case 256: return launch_sets<T, 256>(a, sc, sms, st);
     }
     return cudaErrorInvalidValue;
 }

@@ -203,6 +203,23 @@ def test_attend_lengths_heads_and_layouts(torch, dtype, nq, nkv, hd, page, layou
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nkv,hd", [(17, 1, 64), (24, 2, 192), (40, 1, 128), (33, 1, 256), (10, 1, 64), (16, 1, 192),
+                                       (32, 2, 256)])
+def test_attend_many_heads_on_one(torch, dtype, nq, nkv, hd):
+    """More than eight query heads per kv head share a pass, sixteen at a time; in
+    divided sequences and whole ones, with the weights of all of them."""
+    lengths = [1, 700, 0, 2500]
+    cache = make_cache(torch, 4, 2500, nkv, hd, dtype, 16, seed=nq)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn(4, nq, hd, generator=gen, device="cuda")
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    w = torch.zeros(4, nkv, cache.capacity, device="cuda")
+    ref, tol, wr, wtol = attend_ref(cache, q, lengths, hd ** -0.5, 0, SPLIT[dtype])
+    check(cache.attend(q, n, hd ** -0.5, weights=w), ref, tol)
+    check(w, wr, wtol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_attend_ignores_what_unseen_slots_hold(torch, dtype):
     """NaN and infinities beyond the length, before the window, on pages of no
     sequence and behind table entries that name no page."""
