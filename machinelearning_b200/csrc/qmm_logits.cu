@@ -75,6 +75,8 @@ __global__ void __launch_bounds__(kLogitThreads, 3) process_logits_kernel(const 
     const int shift = kVec ? (int)(((uintptr_t)x >> 2) & 3) : 0;  // entries before the row's first boundary
     const int v0 = (int)blockIdx.x * slice - shift;                // entry 0 of the slice (may be before the row)
     const int lo = v0 < 0 ? -v0 : 0, hi = min(slice, a.vocab - v0);
+    pdl_launch_dependents();
+    pdl_wait();
     if (hi <= lo) return;
     x += v0;
     y += v0;
@@ -261,10 +263,9 @@ cudaError_t launch_process_logits(const LogitsArgs& a, cudaStream_t st) {
     const cudaError_t e = ensure_dynamic_smem(fn, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(((int64_t)a.vocab + 3 + slice - 1) / slice), a.rows);
-    if (vec) process_logits_kernel<true><<<grid, kLogitThreads, smem, st>>>(a, slice);
-    else process_logits_kernel<false><<<grid, kLogitThreads, smem, st>>>(a, slice);
-    note_launch();
-    return cudaGetLastError();
+    LogitsArgs aa = a;
+    void* args[] = {&aa, &slice};
+    return launch_pdl_kernel(fn, grid, dim3(kLogitThreads), smem, st, args);
 }
 
 }  // namespace qmm

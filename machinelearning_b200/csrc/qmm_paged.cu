@@ -43,6 +43,8 @@ __global__ void __launch_bounds__(kAppendThreads, 8) paged_append_kernel(const A
     const int token = blockIdx.x, head = blockIdx.y * (kAppendThreads / G) + threadIdx.x / G;
     const bool is_q = head < a.nq, is_v = head >= a.nq + a.kv.nkv;
     const bool live = lane4 < half && head < a.nq + 2 * a.kv.nkv;
+    pdl_launch_dependents();
+    pdl_wait();
     float4 x = make_float4(0, 0, 0, 0), y = x;
     if (live) {
         const float* src = a.qkv + token * a.ld + (head * hd + lane4);
@@ -109,10 +111,12 @@ cudaError_t launch_append(const AppendArgs& a, bool interleaved, cudaStream_t st
     const int lanes = a.kv.hd / 8;
     const int G = lanes <= 8 ? 8 : (lanes <= 16 ? 16 : 32), groups = kAppendThreads / G;
     const dim3 grid(a.tokens, (a.nq + 2 * a.kv.nkv + groups - 1) / groups);
-    if (interleaved) paged_append_kernel<T, true><<<grid, kAppendThreads, 0, st>>>(a, G);
-    else paged_append_kernel<T, false><<<grid, kAppendThreads, 0, st>>>(a, G);
-    note_launch();
-    return cudaGetLastError();
+    AppendArgs aa = a;
+    int g = G;
+    void* args[] = {&aa, &g};
+    return launch_pdl_kernel(interleaved ? (const void*)paged_append_kernel<T, true>
+                                         : (const void*)paged_append_kernel<T, false>,
+                             grid, dim3(kAppendThreads), 0, st, args);
 }
 
 }  // namespace

@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
     const int heads = a.kv.nkv * sc.head_tiles;  // head tiles of a sequence
 
     pdl_launch_dependents();
+    pdl_wait();
 
     // my share: every warp adds up the sequences' steps by itself
     const int B = a.kv.n_seqs, per = (B + 31) / 32;
@@ -755,6 +756,7 @@ __global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
     extern __shared__ float factors[];  // [kHeads][grid]
     __shared__ float4 part[kGroups][kHeads][kCols];
     __shared__ float inv_s[kHeads];
+    pdl_launch_dependents();
     if (blockIdx.x >= join_blocks) {
         if (blockIdx.y == 0) add_weights<T, S, J::kThreads, J::kHeadsAtOnce>(a, sc, blockIdx.x - join_blocks);
         else pdl_wait();
@@ -888,9 +890,10 @@ cudaError_t launch(const AttendArgs& a, Scratch sc, int sms, cudaStream_t st) {
     cudaError_t e = ensure_dynamic_smem((const void*)attend_kernel<T, HD, SETS>, S::kSmem);
     if (e != cudaSuccess) return e;
     sc.grid = sms * S::kCtas;
-    attend_kernel<T, HD, SETS><<<sc.grid, S::kWarps * 32, S::kSmem, st>>>(a, sc);
-    note_launch();
-    e = cudaGetLastError();
+    AttendArgs aa = a;
+    void* args[] = {&aa, &sc};
+    e = launch_pdl_kernel((const void*)attend_kernel<T, HD, SETS>, dim3(sc.grid), dim3(S::kWarps * 32), S::kSmem, st,
+                          args);
     if (e != cudaSuccess) return e;
     const int tiles = a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
     const int heads = a.nq / a.kv.nkv < S::kHeads ? a.nq / a.kv.nkv : S::kHeads;
