@@ -54,34 +54,37 @@ __device__ __forceinline__ uint32_t tf32_rna(float x) {
     return r;
 }
 
-// x as hi + lo of the instruction's operand type: f32 arithmetic on 16-bit or
-// tf32 operands. What is left over is below 2^-16 |x| (bf16), 2^-22 |x|
-// (f16, tf32).
+// f32 values as sums of the instruction's operands: two f16 or tf32 (22 bits),
+// three bf16 (24 bits; two leave 2^-17, and the outputs four times as far from the
+// exact ones as f32 arithmetic does).
 template <typename T>
-__device__ __forceinline__ void split(float x, T* hi, T* lo) {
-    if constexpr (sizeof(T) == 4) {
-        *hi = __uint_as_float(tf32_rna(x));
-        *lo = __uint_as_float(tf32_rna(x - *hi));
-    } else {
-        *hi = f32_to_kv<T>(x);
-        *lo = f32_to_kv<T>(x - kv_to_f32<T>(*hi));
+constexpr int kParts = std::is_same_v<T, __nv_bfloat16> ? 3 : 2;
+
+template <typename T>
+__device__ __forceinline__ void split(float x, T (&part)[kParts<T>]) {
+#pragma unroll
+    for (int i = 0; i < kParts<T>; ++i) {
+        if constexpr (sizeof(T) == 4) part[i] = __uint_as_float(tf32_rna(x));
+        else part[i] = f32_to_kv<T>(x);
+        x -= kv_to_f32<T>(part[i]);
     }
 }
 // The same for two values at once, packed (16-bit types).
 template <typename T>
-__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
-    if constexpr (std::is_same_v<T, __half>) {
-        const __half2 h = __floats2half2_rn(x, y);
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-        *hi = *reinterpret_cast<const uint32_t*>(&h);
-        *lo = *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        const float2 f = __bfloat1622float2(h);
-        const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
-        *hi = *reinterpret_cast<const uint32_t*>(&h);
-        *lo = *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&part)[kParts<T>]) {
+#pragma unroll
+    for (int i = 0; i < kParts<T>; ++i) {
+        if constexpr (std::is_same_v<T, __half>) {
+            const __half2 h = __floats2half2_rn(x, y);
+            const float2 f = __half22float2(h);
+            part[i] = *reinterpret_cast<const uint32_t*>(&h);
+            x -= f.x, y -= f.y;
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            const float2 f = __bfloat1622float2(h);
+            part[i] = *reinterpret_cast<const uint32_t*>(&h);
+            x -= f.x, y -= f.y;
+        }
     }
 }
 __device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22; 0 below 2^-126
@@ -222,8 +225,8 @@ struct Shape {
     static constexpr int kUnit = kSlots * HD * (int)sizeof(T);
     static constexpr int kUnits = 3;
     static constexpr int kWarps = HD <= 64 || (HD <= 128 && SETS == 1) ? 8 : (HD == 192 && SETS == 1 ? 5 : 4);
-    static constexpr int kQBytes = kChunks * 2 * 32 * 16;        // of a set
-    static constexpr bool kQRegs = SETS == 1 && kChunks <= (kWarps == 8 ? 4 : 8);  // Q in registers
+    static constexpr int kQPairs = kChunks * 2 * 32 * 16;        // of a set: first two parts; a third takes half
+    static constexpr int kQBytes = kQPairs + (kParts<T> - 2) * kQPairs / 2;
     static constexpr int kSetup = 163840 / (2 * kUnit);          // a piece's fixed cost in steps: 6 us measured
     static constexpr int kAccRow = HD + 4;                       // floats; spreads the rows over the banks
     static constexpr size_t kSmem =
@@ -252,9 +255,10 @@ constexpr float kSlack = std::is_same_v<T, __half> ? 1.0f : 8.0f;
 //    (f32: 4) consecutive ones, two by two, and pairs two slots' values by byte
 //    permutes (16 bit).
 // S's layout is that of the operand B of V^T P^T: P stays in registers.
-// In S, operand A has 16 rows for the 8 heads of the tile: rows 0-7 are the high,
-// rows 8-15 the low parts of Q, so the products are those of f32 queries with the
-// cache's, at no cost; P's high and low parts take an instruction each. (O = P V
+// In S, operand A has 16 rows for the 8 heads of a set: rows 0-7 are the first,
+// rows 8-15 the second parts of Q, so the products are those of f32 queries with
+// the cache's, at no cost (a third part takes an instruction); P's parts take an
+// instruction each. (O = P V
 // with the parts as rows took as many, but twice the accumulators: 8 warps per SM
 // for 16.) K and V in f32
 // are split too.
@@ -390,25 +394,24 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
             for (int i = 0; i < HD / 32; ++i) {
                 const int d = lane + 32 * i, c = d / kElems, r = d % kElems;
                 const int step = (c >> 2) * 2 + r / (kElems / 2), p = r % (kElems / 2);
-                T hi, lo;
-                split<T>(x[i] * down, &hi, &lo);
-                T* dst = reinterpret_cast<T*>(qs + (j >> 3) * S::kQBytes + (step * 32 + (j & 7) * 4 + (c & 3)) * 16);
+                T part[kParts<T>];
+                split<T>(x[i] * down, part);
+                uint8_t* set = qs + (j >> 3) * S::kQBytes;
+                const int at = step * 32 + (j & 7) * 4 + (c & 3);
+                T* dst = reinterpret_cast<T*>(set + at * 16);
                 if constexpr (sizeof(T) == 4) {
-                    dst[2 * p] = hi;
-                    dst[2 * p + 1] = lo;
+                    dst[2 * p] = part[0];
+                    dst[2 * p + 1] = part[1];
                 } else {
-                    dst[(p >> 1) * 4 + (p & 1)] = hi;
-                    dst[(p >> 1) * 4 + 2 + (p & 1)] = lo;
+                    dst[(p >> 1) * 4 + (p & 1)] = part[0];
+                    dst[(p >> 1) * 4 + 2 + (p & 1)] = part[1];
+                    if constexpr (kParts<T> == 3) reinterpret_cast<T*>(set + S::kQPairs + at * 8)[p] = part[2];
                 }
             }
         }
         __syncthreads();
         const uint8_t* qs_l = qs + lane * 16;
-        uint4 qr[S::kQRegs ? 2 * S::kChunks : 1];
-        if constexpr (S::kQRegs) {
-#pragma unroll
-            for (int j = 0; j < 2 * S::kChunks; ++j) qr[j] = lds16(qs_l + j * 512);
-        }
+        const uint8_t* qs3_l = qs + S::kQPairs + lane * 8;
         float unit[SETS], m[SETS], l[SETS], lc[SETS];
         float* srow[SETS];
         float acc[SETS][HD / 16][4];  // [two columns]: head 2 t, head 2 t + 1 at the first; the same at the second
@@ -432,48 +435,68 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
             issue(i + 1, pages, a.kv.k, spare, false);
             const Pages after = pages_of(i + 2);
             const uint8_t* src = k_src + at * S::kUnit;
-            // scores: two chains of products per 8 slots and set
-            constexpr int kX = kSlots / 4;
-            float x[SETS][kX];
+            static_assert(S::kChunks % 2 == 0, "runs divide a row");
+            // scores: per 8 slots and set two chains of products, of four units of the row at most (the
+            // instruction cuts off where it adds; longer chains were what f32 caches lost most by)
+            constexpr int kX = kSlots / 4, kR = kSlots / 8 < 2 ? 1 : 2, kRun = S::kChunks % 4 == 0 ? 4 : S::kChunks % 3 == 0 ? 3 : 2;
+            float x[SETS][kX] = {};
 #pragma unroll
-            for (int r = 0; r < kSlots / 8; ++r) {
-                float c0[SETS][4] = {}, c1[SETS][4] = {};
+            for (int r0 = 0; r0 < kSlots / 8; r0 += kR) {
 #pragma unroll
-                for (int j = 0; j < S::kChunks; ++j) {
-                    const uint4 k = lds16(src + 8 * r * S::kRow + (j >> 1) * 128 + k_half[j & 1]);
-                    float hi[4], lo[4];
-                    if constexpr (sizeof(T) == 4) {
-                        split<T>(__uint_as_float(k.x), &hi[0], &lo[0]);
-                        split<T>(__uint_as_float(k.y), &hi[1], &lo[1]);
-                        split<T>(__uint_as_float(k.z), &hi[2], &lo[2]);
-                        split<T>(__uint_as_float(k.w), &hi[3], &lo[3]);
+                for (int j0 = 0; j0 < S::kChunks; j0 += kRun) {
+                    float c0[kR][SETS][4] = {}, c1[kR][SETS][4] = {};
+#pragma unroll
+                    for (int j = j0; j < j0 + kRun; ++j) {
+                        uint4 k[kR];
+#pragma unroll
+                        for (int r = 0; r < kR; ++r)
+                            k[r] = lds16(src + 8 * (r0 + r) * S::kRow + (j >> 1) * 128 + k_half[j & 1]);
+#pragma unroll
+                        for (int q = 0; q < SETS; ++q) {
+                            const uint4 qa = lds16(qs_l + q * S::kQBytes + (2 * j) * 512);
+                            const uint4 qb = lds16(qs_l + q * S::kQBytes + (2 * j + 1) * 512);
+                            uint2 ta = make_uint2(0, 0), tb = ta;
+                            if constexpr (kParts<T> == 3) {
+                                ta = *reinterpret_cast<const uint2*>(qs3_l + q * S::kQBytes + (2 * j) * 256);
+                                tb = *reinterpret_cast<const uint2*>(qs3_l + q * S::kQBytes + (2 * j + 1) * 256);
+                            }
+#pragma unroll
+                            for (int r = 0; r < kR; ++r) {
+                                if constexpr (sizeof(T) == 4) {
+                                    float f0[2], f1[2], f2[2], f3[2];
+                                    split<T>(__uint_as_float(k[r].x), f0);
+                                    split<T>(__uint_as_float(k[r].y), f1);
+                                    split<T>(__uint_as_float(k[r].z), f2);
+                                    split<T>(__uint_as_float(k[r].w), f3);
+#pragma unroll
+                                    for (int e = 1; e >= 0; --e) {
+                                        mma<T>(c0[r][q], qa, __float_as_uint(f0[e]), __float_as_uint(f1[e]));
+                                        mma<T>(c1[r][q], qb, __float_as_uint(f2[e]), __float_as_uint(f3[e]));
+                                    }
+                                } else {
+                                    if constexpr (kParts<T> == 3) {
+                                        mma<T>(c0[r][q], make_uint4(ta.x, 0, ta.y, 0), k[r].x, k[r].y);
+                                        mma<T>(c1[r][q], make_uint4(tb.x, 0, tb.y, 0), k[r].z, k[r].w);
+                                    }
+                                    mma<T>(c0[r][q], qa, k[r].x, k[r].y);
+                                    mma<T>(c1[r][q], qb, k[r].z, k[r].w);
+                                }
+                            }
+                        }
                     }
 #pragma unroll
-                    for (int q = 0; q < SETS; ++q) {
-                        uint4 qa, qb;
-                        if constexpr (S::kQRegs) {
-                            qa = qr[2 * j], qb = qr[2 * j + 1];
-                        } else {
-                            qa = lds16(qs_l + q * S::kQBytes + (2 * j) * 512);
-                            qb = lds16(qs_l + q * S::kQBytes + (2 * j + 1) * 512);
-                        }
-                        if constexpr (sizeof(T) == 4) {
-                            mma<T>(c0[q], qa, __float_as_uint(hi[0]), __float_as_uint(hi[1]));
-                            mma<T>(c1[q], qb, __float_as_uint(hi[2]), __float_as_uint(hi[3]));
-                            mma<T>(c0[q], qa, __float_as_uint(lo[0]), __float_as_uint(lo[1]));
-                            mma<T>(c1[q], qb, __float_as_uint(lo[2]), __float_as_uint(lo[3]));
-                        } else {
-                            mma<T>(c0[q], qa, k.x, k.y);
-                            mma<T>(c1[q], qb, k.z, k.w);
-                        }
-                    }
-                }
+                    for (int r = 0; r < kR; ++r)
 #pragma unroll
-                for (int q = 0; q < SETS; ++q) {
-                    x[q][2 * r] = ((c0[q][0] + c1[q][0]) + (c0[q][2] + c1[q][2])) * unit[q];
-                    x[q][2 * r + 1] = ((c0[q][1] + c1[q][1]) + (c0[q][3] + c1[q][3])) * unit[q];
+                        for (int q = 0; q < SETS; ++q) {
+                            x[q][2 * (r0 + r)] += (c0[r][q][0] + c1[r][q][0]) + (c0[r][q][2] + c1[r][q][2]);
+                            x[q][2 * (r0 + r) + 1] += (c0[r][q][1] + c1[r][q][1]) + (c0[r][q][3] + c1[r][q][3]);
+                        }
                 }
             }
+#pragma unroll
+            for (int q = 0; q < SETS; ++q)
+#pragma unroll
+                for (int r = 0; r < kX; ++r) x[q][r] *= unit[q];
             // lane (g, t) has the scores of heads g, g + 8 at slots 2 t, 2 t + 1 of every eight
             const int slot0 = my_slot0 + i * (W * kSlots);
             bool whole = slot0 >= s.first && slot0 + kSlots <= s.n;
@@ -489,7 +512,7 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                         for (int q = 0; q < SETS; ++q) x[q][r] = -INFINITY;
                 }
             }
-            uint4 p[SETS][kTiles];  // operand B: high parts x, y, low parts z, w
+            uint2 p[SETS][kTiles][kParts<T>];  // operand B of each part
 #pragma unroll
             for (int q = 0; q < SETS; ++q) {
                 if (srow[q]) {
@@ -532,14 +555,18 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
 #pragma unroll
                 for (int u = 0; u < kTiles; ++u) {
                     if constexpr (sizeof(T) == 4) {
-                        float hi[2], lo[2];
-                        split<T>(x[q][2 * u], &hi[0], &lo[0]);
-                        split<T>(x[q][2 * u + 1], &hi[1], &lo[1]);
-                        p[q][u] = make_uint4(__float_as_uint(hi[0]), __float_as_uint(hi[1]), __float_as_uint(lo[0]),
-                                             __float_as_uint(lo[1]));
+                        float f0[2], f1[2];
+                        split<T>(x[q][2 * u], f0);
+                        split<T>(x[q][2 * u + 1], f1);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            p[q][u][e] = make_uint2(__float_as_uint(f0[e]), __float_as_uint(f1[e]));
                     } else {
-                        split2<T>(x[q][4 * u], x[q][4 * u + 1], &p[q][u].x, &p[q][u].z);
-                        split2<T>(x[q][4 * u + 2], x[q][4 * u + 3], &p[q][u].y, &p[q][u].w);
+                        uint32_t f0[kParts<T>], f1[kParts<T>];
+                        split2<T>(x[q][4 * u], x[q][4 * u + 1], f0);
+                        split2<T>(x[q][4 * u + 2], x[q][4 * u + 3], f1);
+#pragma unroll
+                        for (int e = 0; e < kParts<T>; ++e) p[q][u][e] = make_uint2(f0[e], f1[e]);
                     }
                 }
             }
@@ -562,20 +589,20 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                         // high V with both parts of P, low V with the high one: the rest is below 2^-22
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float hi[4], lo[4];
-                            split<T>(__uint_as_float(v0[2 * e]), &hi[0], &lo[0]);
-                            split<T>(__uint_as_float(v0[2 * e + 1]), &hi[1], &lo[1]);
-                            split<T>(__uint_as_float(v1[2 * e]), &hi[2], &lo[2]);
-                            split<T>(__uint_as_float(v1[2 * e + 1]), &hi[3], &lo[3]);
-                            const uint4 vh = make_uint4(__float_as_uint(hi[0]), __float_as_uint(hi[1]),
-                                                        __float_as_uint(hi[2]), __float_as_uint(hi[3]));
-                            const uint4 vl = make_uint4(__float_as_uint(lo[0]), __float_as_uint(lo[1]),
-                                                        __float_as_uint(lo[2]), __float_as_uint(lo[3]));
+                            float f[4][2];
+                            split<T>(__uint_as_float(v0[2 * e]), f[0]);
+                            split<T>(__uint_as_float(v0[2 * e + 1]), f[1]);
+                            split<T>(__uint_as_float(v1[2 * e]), f[2]);
+                            split<T>(__uint_as_float(v1[2 * e + 1]), f[3]);
+                            const uint4 vh = make_uint4(__float_as_uint(f[0][0]), __float_as_uint(f[1][0]),
+                                                        __float_as_uint(f[2][0]), __float_as_uint(f[3][0]));
+                            const uint4 vl = make_uint4(__float_as_uint(f[0][1]), __float_as_uint(f[1][1]),
+                                                        __float_as_uint(f[2][1]), __float_as_uint(f[3][1]));
 #pragma unroll
                             for (int q = 0; q < SETS; ++q) {
-                                mma<T>(acc[q][j * 2 + e], vh, p[q][u].x, p[q][u].y);
-                                mma<T>(acc[q][j * 2 + e], vl, p[q][u].x, p[q][u].y);
-                                mma<T>(acc[q][j * 2 + e], vh, p[q][u].z, p[q][u].w);
+                                mma<T>(acc[q][j * 2 + e], vl, p[q][u][0].x, p[q][u][0].y);
+                                mma<T>(acc[q][j * 2 + e], vh, p[q][u][1].x, p[q][u][1].y);
+                                mma<T>(acc[q][j * 2 + e], vh, p[q][u][0].x, p[q][u][0].y);
                             }
                         }
                     } else {
@@ -588,10 +615,10 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                                                         __byte_perm(v2[e], v3[e], 0x5410),
                                                         __byte_perm(v2[e], v3[e], 0x7632));
 #pragma unroll
-                            for (int q = 0; q < SETS; ++q) {
-                                mma<T>(acc[q][j * 4 + e], vv, p[q][u].x, p[q][u].y);
-                                mma<T>(acc[q][j * 4 + e], vv, p[q][u].z, p[q][u].w);
-                            }
+                            for (int q = 0; q < SETS; ++q)
+#pragma unroll
+                                for (int f = kParts<T> - 1; f >= 0; --f)
+                                    mma<T>(acc[q][j * 4 + e], vv, p[q][u][f].x, p[q][u][f].y);
                         }
                     }
                 }

@@ -71,9 +71,9 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None,
             raise ValueError("rows of logits and out have to be contiguous")
     one, bias = (rows,), (rows, n_bias)
     lib = _lib.lib()
-    with _HERE if torch.cuda.current_device() == dev else torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty((rows, vocab), dtype=f32, device=logits.device)
+    if out is None:
+        out = logits.new_empty((rows, vocab))
+    with _HERE if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev):
         status = lib.qmm_process_logits_dev(
             logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
             _ptr(tokens, "tokens", i32, (rows, width), dev), width, width,

@@ -20,7 +20,6 @@ one dense f32 cache per sequence (layers/main/src/core/attention.rs:454-610).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -29,9 +28,6 @@ from . import _lib
 from ._lib import KV_BF16, KV_F16, KV_F32
 
 KV_DTYPES = {torch.float32: KV_F32, torch.float16: KV_F16, torch.bfloat16: KV_BF16}
-
-
-_HERE = contextlib.nullcontext()
 
 
 def _mismatch(message: str) -> _lib.ShapeMismatch:
@@ -104,13 +100,15 @@ class PagedKVCache:
         raise ValueError(f"{name}: rows have to be contiguous")
 
     def _call(self, fn, *args) -> None:
-        status = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(self._index))
+        """Calls a library function on the current stream of the cache's device (it launches on the
+        current device, which is made the cache's)."""
+        if torch._C._cuda_getDevice() == self._index:
+            status = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(self._index))
+        else:
+            with torch.cuda.device(self.device):
+                status = fn(self._ref, *args, torch._C._cuda_getCurrentRawStream(self._index))
         if status:
             _lib.check(status)
-
-    def _on_device(self):
-        """The library launches on the current device: a context that makes it the cache's."""
-        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)
 
     # ---- operators ---------------------------------------------------------------------
     def append(self, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, cos: torch.Tensor,
@@ -134,15 +132,17 @@ class PagedKVCache:
         i32, f32, check, one = torch.int32, torch.float32, self._check, (tokens,)
         ptr, ld = self._rows(qkv, "qkv", row)
         shape, table = (tokens, n_heads, hd), (ctx, hd // 2)
-        with self._on_device():
-            if out is None:
-                out = torch.empty(shape, dtype=f32, device=self.device)
-            self._call(self._lib.qmm_paged_append_dev, ptr, ld, tokens, n_heads,
-                       None if q_norm is None else check(q_norm, "q_norm", f32, (hd,)),
-                       None if k_norm is None else check(k_norm, "k_norm", f32, (hd,)), offset, eps,
-                       check(cos, "cos", f32, table), check(sin, "sin", f32, table), ctx, int(interleaved),
-                       check(positions, "positions", i32, one), check(slots, "slots", i32, one),
-                       None if seqs is None else check(seqs, "seqs", i32, one), check(out, "out", f32, shape))
+        if out is None:
+            out = qkv.new_empty(shape)
+            out_ptr = out.data_ptr()
+        else:
+            out_ptr = check(out, "out", f32, shape)
+        self._call(self._lib.qmm_paged_append_dev, ptr, ld, tokens, n_heads,
+                   None if q_norm is None else check(q_norm, "q_norm", f32, (hd,)),
+                   None if k_norm is None else check(k_norm, "k_norm", f32, (hd,)), offset, eps,
+                   check(cos, "cos", f32, table), check(sin, "sin", f32, table), ctx, interleaved,
+                   check(positions, "positions", i32, one), check(slots, "slots", i32, one),
+                   None if seqs is None else check(seqs, "seqs", i32, one), out_ptr)
         return out
 
     def attend(self, q: torch.Tensor, lengths: torch.Tensor, scale: float, *, window: int = 0,
@@ -164,12 +164,13 @@ class PagedKVCache:
             w_out = w if weights_out is None else check(weights_out, "weights_out", f32, self._slots_shape)
         elif weights_out is not None:
             raise ValueError("weights_out without weights")
-        with self._on_device():
-            if out is None:
-                out = torch.empty(shape, dtype=f32, device=self.device)
-            self._call(self._lib.qmm_paged_attention_dev, ptr, ld, shape[1],
-                       check(lengths, "lengths", torch.int32, self._seqs_shape), scale, window, w, w_out,
-                       check(out, "out", f32, shape))
+        if out is None:
+            out = q.new_empty(shape)
+            out_ptr = out.data_ptr()
+        else:
+            out_ptr = check(out, "out", f32, shape)
+        self._call(self._lib.qmm_paged_attention_dev, ptr, ld, shape[1],
+                   check(lengths, "lengths", torch.int32, self._seqs_shape), scale, window, w, w_out, out_ptr)
         return out
 
     def evict(self, lengths: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor,
@@ -184,9 +185,8 @@ class PagedKVCache:
         args = (check(lengths, "lengths", i32, self._seqs_shape), check(weights, "weights", f32, slots),
                 check(positions, "positions", i32, slots),
                 check(next_positions, "next_positions", i32, self._seqs_shape), budget, recent)
-        with self._on_device():
-            new = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(positions)
-            self._call(self._lib.qmm_paged_evict_dev, *args, new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr())
+        new = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(positions)
+        self._call(self._lib.qmm_paged_evict_dev, *args, new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr())
         return new
 
     def reserve(self, n_heads: int, weights: bool = False, budget: int = 0,

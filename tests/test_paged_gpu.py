@@ -8,8 +8,8 @@ Tolerances, u = 2^-24 (f32), t = the cache type's unit roundoff (f32 0, f16
   products: at most 16 u of the rotated pair's |a| + |b|, 1.5e-6 with a margin;
   cache rows add t |x| (and half of f16's smallest subnormal).
 * attend: a score is off by at most e = scale * sum |q k| * (r + head_dim u) with r the
-  residue of q held as two values of the matrix instructions' type (bf16 2^-16,
-  f16 and tf32 2^-21); a weight by a relative 2 e + r + 2^-20 (exponentials and the
+  residue of q held as values of the matrix instructions' type (two f16 or tf32
+  2^-21, three bf16 less); a weight by a relative 2 e + r + 2^-20 (exponentials and the
   running sums), so an output by that times sum p |v|.
 * evict: moves and choices: equal.
 * logits: at most eight roundings of values no larger than |x| max(r, 1/r) + f count + p
@@ -24,7 +24,7 @@ pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 ROUNDOFF = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
-SPLIT = {"f32": 2.0 ** -21, "f16": 2.0 ** -21, "bf16": 2.0 ** -16}
+SPLIT = {"f32": 2.0 ** -21, "f16": 2.0 ** -21, "bf16": 2.0 ** -21}
 HEADS = [(4, 1, 256), (64, 8, 128), (15, 3, 64), (16, 1, 128), (12, 2, 192), (1, 1, 64), (9, 1, 256), (8, 8, 64)]
 
 
