@@ -1138,6 +1138,8 @@ QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, 
         if (a.kv.n_seqs == 0) return QMM_OK;
         if (!q_dev || !lengths_dev || !out_dev || (weights_dev == nullptr) != (weights_out_dev == nullptr))
             return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+        if ((long long)a.kv.n_seqs * n_heads > INT32_MAX)
+            return fail(QMM_ERR_SHAPE_MISMATCH, "more than 2^31 - 1 (sequence, query head) rows");
         if (ld_q < (size_t)n_heads * a.kv.hd || window < 0)
             return fail(QMM_ERR_SHAPE_MISMATCH, "query row stride or window out of range");
         if (!aligned16(q_dev) || ld_q % 4 || !aligned16(out_dev) || !aligned16(weights_dev) ||

@@ -135,7 +135,7 @@ template <int kSlots>
 __device__ __forceinline__ Slots slots_of(const AttendArgs& a, int b) {
     Slots s;
     const int64_t cap = a.kv.capacity();
-    const int len = a.lengths[b];
+    const int len = __ldcg(a.lengths + b);  // from L2: join_kernel reads it before its wait
     s.n = len < 0 ? 0 : (len > cap ? (int)cap : len);
     s.first = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
     s.tile0 = s.first / kSlots;
@@ -289,8 +289,10 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
     const int group = a.nq / a.kv.nkv;
     const int heads = a.kv.nkv * sc.head_tiles;  // head tiles of a sequence
 
-    pdl_launch_dependents();
+    // join_kernel reads the lengths and the running weights before it waits for this kernel: it may start
+    // only once all that came before has ended, the last join among it
     pdl_wait();
+    pdl_launch_dependents();
 
     // my share: every warp adds up the sequences' steps by itself
     const int B = a.kv.n_seqs, per = (B + 31) / 32;
@@ -692,8 +694,9 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
 // pieces, eight where there are many. A thread sums four columns
 // of a head over every kGroups-th piece.
 // It is on the way of every small call, so it is launched early (programmatic
-// dependent launch), finds the pieces from the lengths before it waits for
-// attend_kernel, and has one round of loads after it.
+// dependent launch, once attend_kernel's own wait is over), finds the pieces from
+// the lengths before it waits for attend_kernel, and has one round of loads after
+// it.
 // With weights, the CTAs from join_blocks on add the slots' weights.
 template <int HD, int kHeads>
 struct JoinShape {
@@ -720,7 +723,7 @@ __device__ __forceinline__ void add_weights(const AttendArgs& a, const Scratch& 
     const bool mine = t < cap && t < s.n && t + 4 > s.first;
     const bool copy = t < cap && !mine && a.weights_out != a.weights;
     float4 w = make_float4(0, 0, 0, 0);
-    if (mine || copy) w = *reinterpret_cast<const float4*>(a.weights + at);
+    if (mine || copy) w = __ldcg(reinterpret_cast<const float4*>(a.weights + at));
     if (copy) *reinterpret_cast<float4*>(a.weights_out + at) = w;
     pdl_wait();
     if (s.tiles == 0) return;
@@ -790,7 +793,7 @@ __global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
         return;
     }
     const int heads = a.kv.nkv * sc.head_tiles;
-    const int b = blockIdx.x / heads, h = blockIdx.x - b * heads;
+    const int b = blockIdx.x / (unsigned)heads, h = blockIdx.x - b * (unsigned)heads;
     const int group = a.nq / a.kv.nkv;
     const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * S::kHeads;
     const int j0 = blockIdx.y * kHeads, nh = min(kHeads, min(S::kHeads, group - q0) - j0);
@@ -901,8 +904,8 @@ size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Scra
 template <typename T, int HD, int SETS, int kHeads>
 cudaError_t launch_join(AttendArgs a, Scratch sc, int grid_y, cudaStream_t st) {
     using J = JoinShape<HD, kHeads>;
-    unsigned join_blocks = (unsigned)(a.kv.n_seqs * a.kv.nkv * sc.head_tiles);
-    int64_t blocks = join_blocks;
+    int64_t blocks = (int64_t)a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
+    unsigned join_blocks = (unsigned)blocks;
     if (a.weights)
         blocks += (int64_t)a.kv.n_seqs * a.kv.nkv * ((a.kv.capacity() / 4 + J::kThreads - 1) / J::kThreads);
     if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
@@ -922,10 +925,10 @@ cudaError_t launch(const AttendArgs& a, Scratch sc, int sms, cudaStream_t st) {
     e = launch_pdl_kernel((const void*)attend_kernel<T, HD, SETS>, dim3(sc.grid), dim3(S::kWarps * 32), S::kSmem, st,
                           args);
     if (e != cudaSuccess) return e;
-    const int tiles = a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
+    const int64_t tiles = (int64_t)a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
     const int heads = a.nq / a.kv.nkv < S::kHeads ? a.nq / a.kv.nkv : S::kHeads;
     // few head tiles: their heads side by side
-    if ((int64_t)tiles * heads <= 8 * sms) return launch_join<T, HD, SETS, 1>(a, sc, heads, st);
+    if (tiles * heads <= 8 * sms) return launch_join<T, HD, SETS, 1>(a, sc, heads, st);
     return launch_join<T, HD, SETS, 8>(a, sc, SETS, st);
 }
 

@@ -326,6 +326,25 @@ def test_offsets_beyond_32_bits(torch):
     assert torch.equal(v[table[0].long()].transpose(0, 1).reshape(nkv, 256, hd)[:, :100], rows)
 
 
+@pytest.mark.parametrize("n", [90, 20000])
+def test_attend_back_to_back_accumulations(torch, n):
+    """Calls whose launches overlap: each adds its weights to what the one before left."""
+    cache = make_cache(torch, 3, n, 2, 128, "bf16", seed=n)
+    q = torch.randn(3, 8, 128, device="cuda")
+    lengths = torch.tensor([n, n // 2, 1], dtype=torch.int32, device="cuda")
+    one = torch.zeros(3, 2, cache.capacity, device="cuda")
+    cache.attend(q, lengths, 0.1, weights=one)
+    torch.cuda.synchronize()
+    want = torch.zeros_like(one)
+    for _ in range(200):
+        want += one
+    for _ in range(3):
+        many = torch.zeros_like(one)
+        for _ in range(200):
+            cache.attend(q, lengths, 0.1, weights=many)
+        assert torch.equal(many, want)
+
+
 def test_attend_on_another_stream_and_in_a_graph(torch):
     cache = make_cache(torch, 2, 4096, 2, 128, "bf16", seed=10)
     q = torch.randn(2, 8, 128, device="cuda")
