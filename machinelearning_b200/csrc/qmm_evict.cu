@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
     __shared__ __align__(16) int counts[4][kDigits];             // of this CTA, per digit round
     __shared__ int warp_sums[32];
     __shared__ int s_digit, s_left;
+    pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.y, rank = kCluster ? (int)blockIdx.x : 0;
     const int64_t cap = a.kv.capacity(), base = row * cap;
@@ -289,6 +290,7 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveCtas) move_kernel(const Evi
     constexpr int kMoves = 8 / kSteps;  // with their loads in flight together
     const int lane = threadIdx.x & 31;
     const int64_t cap = a.kv.capacity();
+    pdl_launch_dependents();
     pdl_wait();
     // each lane adds up a run of rows
     const int per = (ls.rows + 31) / 32, r0 = lane * per, r1 = min(ls.rows, r0 + per);
@@ -412,13 +414,15 @@ cudaError_t launch_paged_evict(const EvictArgs& a0, void* ws, cudaStream_t st) {
     cfg.gridDim = dim3(ls.ctas, (unsigned)rows);
     cfg.blockDim = dim3(kSelectThreads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)ls.ctas;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ls.ctas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = ls.ctas > 1 ? 1 : 0;
+    cfg.numAttrs = ls.ctas > 1 ? 2 : 1;
     cudaError_t e;
     if (ls.ctas == 1) e = cudaLaunchKernelEx(&cfg, select_kernel<false, true>, a, ls);
     else if (ls.range <= kRound) e = cudaLaunchKernelEx(&cfg, select_kernel<true, true>, a, ls);
