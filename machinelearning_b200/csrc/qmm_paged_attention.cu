@@ -177,20 +177,23 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
     return v;
 }
 
-// The CTAs that hold the pieces of (sequence b, head tile h).
+// The CTAs that hold the pieces of a (sequence, head tile).
 struct Pieces {
     int first, count;
     // Slot of piece p among the CTAs' slots.
     __device__ __forceinline__ int64_t slot(int p) const { return p == 0 ? 2 * first + 1 : 2 * (first + p); }
 };
+// base: the unit of the first step.
+__device__ __forceinline__ Pieces pieces_of(int64_t base, int tiles, int64_t share) {
+    const int64_t first = base / share, last = (base + tiles - 1) / share;
+    return Pieces{(int)first, (int)(last - first) + 1};
+}
 struct Place {
     int64_t start, share;  // unit at which the sequence starts, units per CTA
     int tiles;
     template <typename S>
     __device__ __forceinline__ Pieces pieces(int h) const {
-        const int64_t base = start + (int64_t)h * (tiles + S::kSetup) + S::kSetup;
-        const int64_t first = base / share, last = (base + tiles - 1) / share;
-        return Pieces{(int)first, (int)(last - first) + 1};
+        return pieces_of(start + (int64_t)h * (tiles + S::kSetup) + S::kSetup, tiles, share);
     }
 };
 template <typename S>
@@ -234,6 +237,46 @@ struct Shape {
     static constexpr int kCtas = 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;  // per SM
     static_assert(kHeads * kAccRow * 4 <= kUnits * kUnit, "a warp's result fits in its ring");
 };
+
+// The (sequence, head tile) that unit share * nth + shift of the list belongs to;
+// b < 0: none. Every warp adds up the sequences' units by itself, a lane a run of
+// them.
+struct Found {
+    int64_t share, base;  // base: the unit of the first step of (b, h)
+    int b, h;
+    Slots s;
+};
+template <typename S>
+__device__ __forceinline__ Found find(const AttendArgs& a, const Scratch& sc, int64_t nth, int shift) {
+    const int lane = threadIdx.x & 31, heads = a.kv.nkv * sc.head_tiles;
+    const int B = a.kv.n_seqs, per = (B + 31) / 32;
+    int64_t mine = 0;
+    for (int b = lane * per; b < min(B, (lane + 1) * per); ++b) mine += units_of<S>(slots_of<S::kSlots>(a, b), heads);
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += u;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    Found f;
+    f.share = share_of<S>(total, sc.grid);
+    f.b = -1;
+    const int64_t unit = f.share * nth + shift;
+    if (unit >= total) return f;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, unit >= before && unit < before + mine)) - 1;
+    f.b = owner * per;
+    int64_t off = unit - __shfl_sync(0xffffffffu, before, owner);
+    f.s = slots_of<S::kSlots>(a, f.b);
+    while (off >= units_of<S>(f.s, heads)) {
+        off -= units_of<S>(f.s, heads);
+        f.s = slots_of<S::kSlots>(a, ++f.b);
+    }
+    f.h = (int)(off / (f.s.tiles + S::kSetup));
+    f.base = unit - (off - (int64_t)f.h * (f.s.tiles + S::kSetup)) + S::kSetup;
+    return f;
+}
 
 // Weights are relative to 2^m with m at most kSlack below the largest score so
 // far (in units of log 2): the sums are rescaled when it grows by more, not at
@@ -294,32 +337,12 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
     pdl_wait();
     pdl_launch_dependents();
 
-    // my share: every warp adds up the sequences' steps by itself
-    const int B = a.kv.n_seqs, per = (B + 31) / 32;
-    int64_t mine = 0;
-    for (int b = lane * per; b < min(B, (lane + 1) * per); ++b) mine += units_of<S>(slots_of<kSlots>(a, b), heads);
-    int64_t before = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += u;
-    }
-    const int64_t total = __shfl_sync(0xffffffffu, before, 31);
-    before -= mine;
-    const int64_t share = share_of<S>(total, gridDim.x);
-    const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
-    if (begin >= end) return;
-    const int owner = __ffs(__ballot_sync(0xffffffffu, begin >= before && begin < before + mine)) - 1;
-    int b = owner * per;
-    int64_t off = begin - __shfl_sync(0xffffffffu, before, owner);
-    Slots s = slots_of<kSlots>(a, b);
-    while (off >= units_of<S>(s, heads)) {
-        off -= units_of<S>(s, heads);
-        s = slots_of<kSlots>(a, ++b);
-    }
-    int h = (int)(off / (s.tiles + S::kSetup));
-    // where the steps of (b, h) begin in the list
-    int64_t base = begin - (off - (int64_t)h * (s.tiles + S::kSetup)) + S::kSetup;
+    const Found found = find<S>(a, sc, blockIdx.x, 0);
+    if (found.b < 0) return;
+    const int64_t share = found.share, begin = share * blockIdx.x, end = begin + share;
+    int b = found.b, h = found.h;
+    int64_t base = found.base;
+    Slots s = found.s;
 
     while (base < end) {
         const int tile = (int)max(begin - base, (int64_t)0);
@@ -681,18 +704,22 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
         if (base >= end) return;
         if (++h == heads) {
             h = 0;
-            do s = slots_of<kSlots>(a, ++b);
-            while (s.tiles == 0);
+            do {
+                if (++b == a.kv.n_seqs) return;
+                s = slots_of<kSlots>(a, b);
+            } while (s.tiles == 0);
         }
         __syncthreads();  // the rings and Q are rewritten
     }
 }
 
 // Joins the pieces of divided (sequence, head tile)s in the order of the CTAs
-// that left them, and writes the zeros of sequences without slots. A CTA takes
-// kHeads heads of a head tile: one where there are few head tiles with many
-// pieces, eight where there are many. A thread sums four columns
-// of a head over every kGroups-th piece.
+// that left them, and writes the zeros of sequences without slots. Few head tiles
+// with many pieces: a CTA per head (kHeads 1). Many head tiles: a CTA per CTA of
+// attend_kernel, for the one head tile at most that it begins and does not end,
+// eight heads at once (256 sequences of up to 300 slots, 64/8 heads of 128: a CTA
+// per head tile took 4 us longer to find that it had nothing to do). A thread sums
+// four columns of a head over every kGroups-th piece.
 // It is on the way of every small call, so it is launched early (programmatic
 // dependent launch, once attend_kernel's own wait is over), finds the pieces from
 // the lengths before it waits for attend_kernel, and has one round of loads after
@@ -792,24 +819,38 @@ __global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
         else pdl_wait();
         return;
     }
-    const int heads = a.kv.nkv * sc.head_tiles;
-    const int b = blockIdx.x / (unsigned)heads, h = blockIdx.x - b * (unsigned)heads;
     const int group = a.nq / a.kv.nkv;
-    const int kvh = h / sc.head_tiles, q0 = (h - kvh * sc.head_tiles) * S::kHeads;
-    const int j0 = blockIdx.y * kHeads, nh = min(kHeads, min(S::kHeads, group - q0) - j0);
-    const int64_t head0 = (int64_t)b * a.nq + kvh * group + q0 + j0;
     const int unit = threadIdx.x / kCols, col = threadIdx.x - unit * kCols;
     const int grp = unit / kHeads, j = unit - grp * kHeads;
-    const Place place = place_of<S>(a, sc, b);
-    const Pieces pc = place.pieces<S>(h);
-    pdl_wait();
-    if (nh <= 0) return;
-    float4* out = reinterpret_cast<float4*>(a.out + (head0 + j) * HD) + col;
-    if (place.tiles == 0) {
-        if (grp == 0 && j < nh) *out = make_float4(0, 0, 0, 0);
-        return;
+    Found f;
+    bool divided;
+    if constexpr (kHeads == 1) {
+        const int heads = a.kv.nkv * sc.head_tiles;
+        f.b = blockIdx.x / (unsigned)heads;
+        f.h = blockIdx.x - f.b * (unsigned)heads;
+        const Place place = place_of<S>(a, sc, f.b);
+        f.s = slots_of<S::kSlots>(a, f.b);
+        f.share = place.share;
+        f.base = place.start + (int64_t)f.h * (f.s.tiles + S::kSetup) + S::kSetup;
+        divided = f.s.tiles > 0 && place.pieces<S>(f.h).count > 1;
+    } else {  // that of the last unit of CTA c's share
+        f = find<S>(a, sc, (int64_t)blockIdx.x + 1, -1);
+        const int64_t bound = f.share * (blockIdx.x + 1);
+        divided = f.b >= 0 && f.base < bound && f.base + f.s.tiles > bound && f.base / f.share == blockIdx.x;
     }
-    if (pc.count == 1) return;  // written by its CTA
+    pdl_wait();
+    for (int b = blockIdx.x; b < a.kv.n_seqs; b += join_blocks)
+        if (blockIdx.y == 0 && slots_of<S::kSlots>(a, b).tiles == 0) {
+            float4* out = reinterpret_cast<float4*>(a.out + (int64_t)b * a.nq * HD);
+            for (int i = threadIdx.x; i < a.nq * (HD / 4); i += J::kThreads) out[i] = make_float4(0, 0, 0, 0);
+        }
+    if (!divided) return;
+    const Pieces pc = pieces_of(f.base, f.s.tiles, f.share);
+    const int kvh = f.h / sc.head_tiles, q0 = (f.h - kvh * sc.head_tiles) * S::kHeads;
+    const int j0 = blockIdx.y * kHeads, nh = min(kHeads, min(S::kHeads, group - q0) - j0);
+    if (nh <= 0) return;
+    const int64_t head0 = (int64_t)f.b * a.nq + kvh * group + q0 + j0;
+    float4* out = reinterpret_cast<float4*>(a.out + (head0 + j) * HD) + col;
     const bool mine = grp < kGroups && j < nh;
     auto load = [&](int p) {
         return reinterpret_cast<const float4*>(sc.acc + (pc.slot(p) * S::kHeads + j0 + j) * HD)[col];
@@ -904,7 +945,7 @@ size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Scra
 template <typename T, int HD, int SETS, int kHeads>
 cudaError_t launch_join(AttendArgs a, Scratch sc, int grid_y, cudaStream_t st) {
     using J = JoinShape<HD, kHeads>;
-    int64_t blocks = (int64_t)a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
+    int64_t blocks = kHeads == 1 ? (int64_t)a.kv.n_seqs * a.kv.nkv * sc.head_tiles : sc.grid;
     unsigned join_blocks = (unsigned)blocks;
     if (a.weights)
         blocks += (int64_t)a.kv.n_seqs * a.kv.nkv * ((a.kv.capacity() / 4 + J::kThreads - 1) / J::kThreads);
