@@ -123,7 +123,7 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 // e^(m - M) of a piece's maximum m, 0 for a piece that saw no slot.
-__device__ __forceinline__ float piece_factor(float m, float M) { return m == -INFINITY ? 0.0f : exp2f(m - M); }
+__device__ __forceinline__ float piece_factor(float m, float M) { return m == -INFINITY ? 0.0f : ex2(m - M); }
 
 // ---- division of the work -----------------------------------------------------------
 // The slots [first, n) of a sequence, in steps ("tiles") of kSlots aligned slots.
