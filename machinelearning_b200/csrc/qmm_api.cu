@@ -139,8 +139,9 @@ int get_workspace(int dev, void* stream, size_t need, void** out) {
         }
         size_t want = need < (1u << 20) ? (1u << 20) : need;
         QMM_CUDA(cudaMalloc(&b.ptr, want));
-        QMM_CUDA(cudaMemset(b.ptr, 0, want));
         b.bytes = want;
+        // on the call's stream: a clear on another one could reach the buffer while the call uses it
+        QMM_CUDA(cudaMemsetAsync(b.ptr, 0, want, (cudaStream_t)stream));
     }
     *out = b.ptr;
     return QMM_OK;
