@@ -118,31 +118,40 @@ int current_device() {
 struct Buffer {
     void* ptr = nullptr;
     size_t bytes = 0;
+    bool captured = false;  // a CUDA graph holds ptr
 };
 std::mutex g_ws_mu;
 std::map<std::pair<int, void*>, Buffer> g_ws;
 std::map<std::pair<int, void*>, Buffer> g_io;  // host-entry staging (qmm_linear_forward_host)
 
+bool is_capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &cs) == cudaSuccess) return cs != cudaStreamCaptureStatusNone;
+    cudaGetLastError();  // the legacy stream beside a capture: not captured itself
+    return false;
+}
+
 int get_workspace(int dev, void* stream, size_t need, void** out) {
     std::lock_guard<std::mutex> lock(g_ws_mu);
     Buffer& b = g_ws[{dev, stream}];
+    const bool capturing = need && is_capturing((cudaStream_t)stream);
     if (b.bytes < need) {
-        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing((cudaStream_t)stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone)
+        if (capturing)
             return fail(QMM_ERR_INVALID_INPUT,
                         "workspace must grow during stream capture; call qmm_reserve_workspace first");
-        if (b.ptr) {
+        // a buffer whose address a graph holds is never freed: the graph may be replayed at any time
+        if (b.ptr && !b.captured) {
             cudaStreamSynchronize((cudaStream_t)stream);
             cudaFree(b.ptr);
-            b.ptr = nullptr;
-            b.bytes = 0;
         }
+        b = Buffer{};
         size_t want = need < (1u << 20) ? (1u << 20) : need;
         QMM_CUDA(cudaMalloc(&b.ptr, want));
         b.bytes = want;
         // on the call's stream: a clear on another one could reach the buffer while the call uses it
         QMM_CUDA(cudaMemsetAsync(b.ptr, 0, want, (cudaStream_t)stream));
     }
+    b.captured |= capturing;
     *out = b.ptr;
     return QMM_OK;
 }

@@ -53,3 +53,40 @@ def test_a_new_workspace_is_cleared_before_its_first_use(torch, reserve):
     want = cache.evict(n, first, pos, n, budget=cap // 2, recent=10)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(cache.k, moved[0]) and torch.equal(cache.v, moved[1])
+
+
+def test_a_graph_keeps_its_workspace_when_a_later_call_needs_more(torch):
+    """A captured step over a small cache, then a direct call over a large one on the
+    same stream: replays give the same result, and write to nobody else's memory."""
+    stream = torch.cuda.Stream()
+    small = make_cache(torch, 2, 4096, 2, 128, "bf16", seed=2)
+    q = torch.randn(2, 8, 128, device="cuda")
+    n = torch.tensor([4096, 3000], dtype=torch.int32, device="cuda")
+    zero = torch.zeros(2, 2, 4096, device="cuda")
+    out, w = torch.zeros_like(q), zero.clone()
+    large = make_cache(torch, 8, 65536, 8, 64, "bf16", 64, seed=3)  # 268 MB of scores
+    ql = torch.randn(8, 64, 64, device="cuda")
+    nl = torch.full((8,), 65536, dtype=torch.int32, device="cuda")
+    wl = torch.zeros(8, 8, 65536, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        small.reserve(8, weights=True)
+        small.attend(q, n, 0.1, out=out, weights=w, weights_out=w)
+        want = out.clone(), w.clone()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            small.attend(q, n, 0.1, out=out, weights=w, weights_out=w)
+        large.attend(ql, nl, 0.1, weights=wl)
+        stream.synchronize()
+        # whatever was freed is handed out again, in pieces of the sizes of the buffer
+        others = [torch.full((size,), 7.0, device="cuda") for size in (1 << 18, 1 << 20, 1 << 22) for _ in range(8)]
+        for _ in range(3):
+            out.zero_(), w.zero_()
+            graph.replay()
+            stream.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(w, want[1])
+        assert all(bool((t == 7.0).all()) for t in others)
+        again = torch.zeros_like(wl)
+        large.attend(ql, nl, 0.1, weights=again)  # the larger buffer serves the direct calls
+        assert torch.equal(again, wl)
