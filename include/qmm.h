@@ -198,7 +198,8 @@ QMM_API int qmm_weight_checksum(const qmm_weight* w, unsigned long long* out);
  * cudaMalloc; grow it with qmm_reserve_workspace before capturing a graph).
  * A graph keeps the buffer that it was captured with: a later call that needs a
  * larger one gets a new one, and the old one is not freed. Replay the graph on
- * the stream it was captured on, or while nothing else runs there. */
+ * the stream it was captured on, or while nothing else runs there. Host threads
+ * may call on one stream at the same time: the launches of a call stay together. */
 QMM_API int qmm_linear_forward(const qmm_weight* w, const float* x_dev, size_t m, float* y_dev, int act,
                                void* stream);
 /* Host-buffer variant of qmm_linear_forward: copies x in and y out on `stream`

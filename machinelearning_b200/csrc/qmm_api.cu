@@ -119,6 +119,14 @@ struct Buffer {
     void* ptr = nullptr;
     size_t bytes = 0;
     bool captured = false;  // a CUDA graph holds ptr
+    std::mutex in_use;
+};
+// A stream's buffer, its owner's until it goes out of scope. Calls of several
+// launches keep data in it between them, so another host thread's call on the stream
+// has to wait until they are all queued.
+struct Workspace {
+    void* ptr = nullptr;
+    std::unique_lock<std::mutex> lock;
 };
 std::mutex g_ws_mu;
 std::map<std::pair<int, void*>, Buffer> g_ws;
@@ -131,9 +139,14 @@ bool is_capturing(cudaStream_t st) {
     return false;
 }
 
-int get_workspace(int dev, void* stream, size_t need, void** out) {
-    std::lock_guard<std::mutex> lock(g_ws_mu);
-    Buffer& b = g_ws[{dev, stream}];
+int get_workspace(int dev, void* stream, size_t need, Workspace* out) {
+    Buffer* entry;
+    {
+        std::lock_guard<std::mutex> lock(g_ws_mu);
+        entry = &g_ws[{dev, stream}];  // entries stay where they are
+    }
+    Buffer& b = *entry;
+    out->lock = std::unique_lock<std::mutex>(b.in_use);
     const bool capturing = need && is_capturing((cudaStream_t)stream);
     if (b.bytes < need) {
         if (capturing)
@@ -144,7 +157,9 @@ int get_workspace(int dev, void* stream, size_t need, void** out) {
             cudaStreamSynchronize((cudaStream_t)stream);
             cudaFree(b.ptr);
         }
-        b = Buffer{};
+        b.ptr = nullptr;
+        b.bytes = 0;
+        b.captured = false;
         size_t want = need < (1u << 20) ? (1u << 20) : need;
         QMM_CUDA(cudaMalloc(&b.ptr, want));
         b.bytes = want;
@@ -152,7 +167,7 @@ int get_workspace(int dev, void* stream, size_t need, void** out) {
         QMM_CUDA(cudaMemsetAsync(b.ptr, 0, want, (cudaStream_t)stream));
     }
     b.captured |= capturing;
-    *out = b.ptr;
+    out->ptr = b.ptr;
     return QMM_OK;
 }
 
@@ -653,15 +668,15 @@ QMM_API int qmm_gated_forward(const qmm_weight* w, const float* x_dev, size_t m,
     DeviceGuard guard(w->device);
     if (!guard.ok) return fail(QMM_ERR_CUDA, "cudaSetDevice failed");
     const size_t need = workspace_for(w->dtype, QMM_ACT_F32, m, w->n, w->k, w->device);
-    void* ws = nullptr;
+    Workspace ws;
     int rc = get_workspace(w->device, stream, need, &ws);
     if (rc) return rc;
     GatedOut g;
     g.act = act_fn;
     g.out = out_dev;
     g.hidden = (int64_t)w->gate_hidden;
-    return run_matmul(w->dtype, QMM_ACT_F32, x_dev, w->dev, m, w->k, w->n, nullptr, ws, need, (cudaStream_t)stream,
-                      /*immutable_w=*/true, g);
+    return run_matmul(w->dtype, QMM_ACT_F32, x_dev, w->dev, m, w->k, w->n, nullptr, ws.ptr, need,
+                      (cudaStream_t)stream, /*immutable_w=*/true, g);
 }
 
 QMM_API int qmm_weight_destroy(qmm_weight* w) {
@@ -721,8 +736,8 @@ QMM_API size_t qmm_workspace_size(int dtype, int act, size_t m, size_t n, size_t
 QMM_API int qmm_reserve_workspace(int device, void* stream, size_t bytes) {
     DeviceGuard guard(device);
     if (!guard.ok) return fail(QMM_ERR_INVALID_INPUT, "bad device");
-    void* p = nullptr;
-    return get_workspace(device, stream, bytes, &p);
+    Workspace ws;
+    return get_workspace(device, stream, bytes, &ws);
 }
 
 QMM_API int qmm_matmul_dev(int dtype, int act, const float* x_dev, const uint8_t* w_dev, size_t w_len, size_t m,
@@ -748,10 +763,10 @@ QMM_API int qmm_linear_forward(const qmm_weight* w, const float* x_dev, size_t m
     DeviceGuard guard(w->device);
     if (!guard.ok) return fail(QMM_ERR_CUDA, "cudaSetDevice failed");
     const size_t need = workspace_for(w->dtype, act, m, w->n, w->k, w->device);
-    void* ws = nullptr;
+    Workspace ws;
     int rc = get_workspace(w->device, stream, need, &ws);
     if (rc) return rc;
-    return run_matmul(w->dtype, act, x_dev, w->dev, m, w->k, w->n, y_dev, ws, need, (cudaStream_t)stream,
+    return run_matmul(w->dtype, act, x_dev, w->dev, m, w->k, w->n, y_dev, ws.ptr, need, (cudaStream_t)stream,
                       /*immutable_w=*/true);
 }
 
@@ -766,7 +781,7 @@ QMM_API int qmm_linear_forward_host(const qmm_weight* w, const float* x_host, si
     auto al = [](size_t v) { return (v + 255) & ~size_t(255); };
     const size_t ws_need = workspace_for(w->dtype, act, m, w->n, w->k, w->device);
     const size_t io = al(m * w->k * 4) + al(m * w->n * 4);
-    void* ws = nullptr;
+    Workspace ws;  // held until the result is out: the staging buffer is the stream's too
     int rc = get_workspace(w->device, stream, ws_need, &ws);
     if (rc) return rc;
     // staging buffers for x/y live apart from the compute workspace, so a
@@ -792,7 +807,7 @@ QMM_API int qmm_linear_forward_host(const qmm_weight* w, const float* x_host, si
     float* yd = reinterpret_cast<float*>(base + al(m * w->k * 4));
     cudaStream_t st = (cudaStream_t)stream;
     QMM_CUDA(cudaMemcpyAsync(xd, x_host, m * w->k * 4, cudaMemcpyHostToDevice, st));
-    rc = run_matmul(w->dtype, act, xd, w->dev, m, w->k, w->n, yd, ws, ws_need, st, /*immutable_w=*/true);
+    rc = run_matmul(w->dtype, act, xd, w->dev, m, w->k, w->n, yd, ws.ptr, ws_need, st, /*immutable_w=*/true);
     if (rc) return rc;
     QMM_CUDA(cudaMemcpyAsync(y_host, yd, m * w->n * 4, cudaMemcpyDeviceToHost, st));
     QMM_CUDA(cudaStreamSynchronize(st));
@@ -1077,8 +1092,7 @@ int check_heads(int n_heads, const PagedKv& kv) {
     return QMM_OK;
 }
 
-int paged_workspace(size_t need, void* stream, void** ws) {
-    *ws = nullptr;
+int paged_workspace(size_t need, void* stream, Workspace* ws) {
     if (!need) return QMM_OK;
     const int dev = current_device();
     if (dev < 0) return fail(QMM_ERR_NO_DEVICE, "no CUDA device");
@@ -1164,10 +1178,10 @@ QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, 
         a.weights = weights_dev;
         a.weights_out = weights_out_dev;
         a.out = out_dev;
-        void* ws = nullptr;
+        Workspace ws;
         rc = paged_workspace(paged_attention_workspace(a.kv, n_heads, weights_dev != nullptr), stream, &ws);
         if (rc) return rc;
-        const cudaError_t e = launch_paged_attention(a, ws, (cudaStream_t)stream);
+        const cudaError_t e = launch_paged_attention(a, ws.ptr, (cudaStream_t)stream);
         return e == cudaSuccess ? QMM_OK : cuda_fail(e, "paged attention");
     });
 }
@@ -1207,10 +1221,10 @@ QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, 
         a.lengths_out = lengths_out_dev;
         a.weights_out = weights_out_dev;
         a.positions_out = positions_out_dev;
-        void* ws = nullptr;
+        Workspace ws;
         rc = paged_workspace(paged_evict_workspace(a.kv, budget), stream, &ws);
         if (rc) return rc;
-        const cudaError_t e = launch_paged_evict(a, ws, (cudaStream_t)stream);
+        const cudaError_t e = launch_paged_evict(a, ws.ptr, (cudaStream_t)stream);
         return e == cudaSuccess ? QMM_OK : cuda_fail(e, "paged evict");
     });
 }

@@ -90,3 +90,47 @@ def test_a_graph_keeps_its_workspace_when_a_later_call_needs_more(torch):
         again = torch.zeros_like(wl)
         large.attend(ql, nl, 0.1, weights=again)  # the larger buffer serves the direct calls
         assert torch.equal(again, wl)
+
+
+def test_host_threads_on_one_stream(torch, oracle):
+    """Calls of several launches from three host threads on one stream: attention over
+    divided sequences, evictions, and a matmul that sums its K splits in the
+    same workspace. Each has the results that it has alone."""
+    import threading
+
+    import numpy as np
+
+    from machinelearning_b200 import _lib
+    from machinelearning_b200.linear import Linear, QuantWeight
+    jobs = []
+    for i in range(2):
+        cache = make_cache(torch, 2, 8192, 2, 128, "bf16", seed=20 + i)
+        q = torch.randn(2, 8, 128, device="cuda")
+        n = torch.tensor([8192, 5000 - i], dtype=torch.int32, device="cuda")
+        jobs.append(lambda cache=cache, q=q, n=n: cache.attend(q, n, 0.1))
+    spare = make_cache(torch, 4, 2048, 2, 64, "f16", seed=22)
+    w = torch.rand(4, 2, 2048, device="cuda")
+    pos = torch.arange(2048, dtype=torch.int32, device="cuda").expand(4, 2, 2048).contiguous()
+    full = torch.full((4,), 2048, dtype=torch.int32, device="cuda")
+    jobs.append(lambda: torch.cat([t.float().flatten() for t in spare.evict(full, w, pos, full, 1000, 10)]))
+    rng = np.random.default_rng(0)
+    m, k, rows = 20, 1152, 256  # rows of 1224 bytes: the streaming kernel, with K split
+    lin = Linear(QuantWeight.from_host(_lib.Q8_0, rows, k, oracle.quantize_q8_0(
+        rng.normal(0, 0.05, rows * k).astype(np.float32)), device=0))
+    x = torch.from_numpy(rng.normal(0, 1, (m, k)).astype(np.float32)).cuda()
+    jobs.append(lambda: lin(x))
+    want = [job().clone() for job in jobs]
+    wrong = [None] * len(jobs)
+    gate = threading.Barrier(len(jobs))
+
+    def work(i):
+        gate.wait()
+        got = [jobs[i]() for _ in range(300)]
+        wrong[i] = sum(not torch.equal(g, want[i]) for g in got)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [0] * len(jobs)
+    lin.weight.close()
