@@ -23,6 +23,7 @@ replays while the graph itself advances the position.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import dataclasses
 import math
@@ -272,11 +273,21 @@ class Gemma3Decoder:
         if advance:
             self._advance()
 
+    @contextlib.contextmanager
+    def _ordered(self):
+        """The step's stream, after what the caller's stream holds and before what follows there."""
+        caller = torch.cuda.current_stream(self.dev)
+        self.stream.wait_stream(caller)
+        try:
+            with torch.cuda.stream(self.stream):
+                yield
+        finally:
+            caller.wait_stream(self.stream)
+
     def set_position(self, pos: int) -> None:
         if not 0 <= pos < self.cfg.ctx:
             raise ValueError(f"position {pos} outside the cache (0..{self.cfg.ctx - 1})")
-        self.stream.wait_stream(torch.cuda.current_stream(self.dev))
-        with torch.cuda.stream(self.stream):
+        with self._ordered():
             self.pos.fill_(pos)
 
     def set_tokens(self, tokens) -> None:
@@ -298,7 +309,7 @@ class Gemma3Decoder:
             return
         # one direct launch first (it rewrites this position's cache rows with
         # the same values): kernel attributes are set outside the capture
-        with torch.cuda.stream(self.stream):
+        with self._ordered():
             self._launch(False)
         torch.cuda.synchronize(self.dev)
         g = torch.cuda.CUDAGraph()
@@ -312,14 +323,12 @@ class Gemma3Decoder:
         the kernels are launched directly."""
         if tokens is not None:
             self.set_tokens(tokens)
-        if self.graph is not None:
-            with torch.cuda.stream(self.stream):
+        # after what the caller's stream still does with the last step's logits; what it does next sees these
+        with self._ordered():
+            if self.graph is not None:
                 self.graph.replay()
-        else:
-            with torch.cuda.stream(self.stream):
+            else:
                 self._launch(advance)
-        # work queued on the caller's stream after this call sees the logits
-        torch.cuda.current_stream(self.dev).wait_stream(self.stream)
         return self.logits
 
     def wait(self, timeout_s: float = 60.0) -> None:

@@ -12,8 +12,6 @@ one position and a dense f32 cache.
 """
 from __future__ import annotations
 
-import contextlib
-
 import numpy as np
 import torch
 
@@ -66,15 +64,6 @@ class PagedGemma3Decoder(Gemma3Decoder):
         self.penalties = {"repetition": one, "presence": zero.clone(), "frequency": zero.clone()}
         self.bias_ids = self.bias_values = self.mask = self.mask_rows = None
         self.caches[0].reserve(cfg.n_heads, weights=bool(self.budget), budget=self.budget, stream=self.stream)
-
-    @contextlib.contextmanager
-    def _ordered(self):
-        """The step's stream, after what the caller's stream holds and before what follows there."""
-        caller = torch.cuda.current_stream(self.dev)
-        self.stream.wait_stream(caller)
-        with torch.cuda.stream(self.stream):
-            yield
-        caller.wait_stream(self.stream)
 
     # ---- sequences ---------------------------------------------------------------------
     def start(self, seq: int, prompt_length: int = 0) -> None:
