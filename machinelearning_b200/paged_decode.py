@@ -98,7 +98,8 @@ class PagedGemma3Decoder(Gemma3Decoder):
 
     def set_constraints(self, bias_ids=None, bias_values=None, mask=None, mask_rows=None) -> None:
         """Biases and grammar states as ``process_logits`` takes them (None: none). A captured
-        step keeps the tensors it was captured with: change those in place, or capture again."""
+        step goes on with the tensors it was captured with, which it keeps alive: change those in
+        place, or capture again."""
         self.bias_ids, self.bias_values, self.mask, self.mask_rows = bias_ids, bias_values, mask, mask_rows
 
     # ---- one step ----------------------------------------------------------------------
@@ -149,6 +150,7 @@ class PagedGemma3Decoder(Gemma3Decoder):
             for li, w in kept.items():
                 self.slot_weights[li].copy_(w)
         self._captured_advance = advance
+        self._captured_constraints = self.bias_ids, self.bias_values, self.mask, self.mask_rows  # read by replays
 
     def step(self, tokens=None, advance: bool = True) -> torch.Tensor:
         """Processed logits [batch][vocab] of one step of all started sequences (rows of idle

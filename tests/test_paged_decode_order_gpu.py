@@ -63,3 +63,34 @@ def test_the_next_step_waits_for_readers_of_the_last_logits(oracle, torch, paged
     assert all(torch.equal(a, b) for a, b in zip(want, kept))
     assert not torch.equal(want[0], want[1])
     model.close()
+
+
+def test_a_captured_step_keeps_its_constraints_alive(oracle, torch):
+    """Constraints replaced after the capture, with no other reference to the old ones:
+    replays go on with those, whatever the freed memory holds."""
+    import gc
+
+    from machinelearning_b200.paged_decode import PagedGemma3Decoder
+    cfg = small_config()
+    model = PagedGemma3Decoder(cfg, host_weights(oracle, cfg, seed=83), batch=2)
+    words = cfg.vocab // 32
+    mask = torch.zeros(1, words, dtype=torch.int32, device="cuda")
+    mask[0, 3] = -1
+    ids = torch.tensor([[97], [110]], dtype=torch.int32, device="cuda")
+    model.set_constraints(bias_ids=ids, bias_values=torch.full((2, 1), 1e4, device="cuda"), mask=mask,
+                          mask_rows=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    model.start(0), model.start(1)
+    model.capture()
+    del mask, ids
+    model.set_constraints()
+    gc.collect()
+    filled = [torch.full((n,), v, device="cuda", dtype=torch.int32) for n in (1, 2, words, 128) for v in (0, 5, -1)
+              for _ in range(40)]
+    for _ in range(4):
+        model.step([3, 4])
+        assert model.next_tokens.tolist() == [97, 110]
+    assert filled
+    model.capture()  # without constraints now
+    model.step([3, 4])
+    assert torch.equal(model.processed, model.logits)
+    model.close()
