@@ -161,8 +161,11 @@ class PagedGemma3Decoder(Gemma3Decoder):
             advance = self._captured_advance
         super().step(tokens, advance)
         if advance:
-            self.host_positions = [p + (p >= 0) for p in self.host_positions]
+            self._move_on()
         return self.processed
+
+    def _move_on(self) -> None:
+        self.host_positions = [p + (p >= 0) for p in self.host_positions]
 
     def evict(self) -> None:
         """Brings the global layers down to ``budget`` slots a sequence and kv head."""
@@ -179,9 +182,18 @@ class PagedGemma3Decoder(Gemma3Decoder):
 
     def generate(self, prompts: list[list[int]], max_new_tokens: int, evict_every: int = 0) -> list[list[int]]:
         """The most likely continuations of up to ``batch`` prompts, fed one token a step and
-        each sequence's own tokens from there on; with a budget, evicts every so many steps."""
+        each sequence's own tokens from there on; with a budget, evicts every so many steps.
+        Begins the first sequences anew, one a prompt, and leaves them idle; the others have to be."""
         if len(prompts) > self.batch or any(not p for p in prompts):
-            raise ValueError(f"1 to {self.batch} prompts of at least one token")
+            raise ValueError(f"at most {self.batch} prompts, of at least one token")
+        if max_new_tokens < 0 or any(len(p) + max_new_tokens - 1 > self.cfg.ctx for p in prompts):
+            raise ValueError(f"a prompt and {max_new_tokens} new tokens exceed {self.cfg.ctx} positions")
+        if evict_every and not self.budget:
+            raise ValueError("no cache budget to evict to")
+        if not prompts or not max_new_tokens:
+            return [[] for _ in prompts]
+        if any(p >= 0 for p in self.host_positions[len(prompts):]):
+            raise ValueError("a sequence without a prompt is started: it would be fed tokens of nobody's")
         for s, p in enumerate(prompts):
             self.start(s, len(p))
         out: list[list[int]] = [[] for _ in prompts]
@@ -193,6 +205,10 @@ class PagedGemma3Decoder(Gemma3Decoder):
                 if 0 <= self.host_positions[s] < len(p):
                     tokens[s] = p[self.host_positions[s]]
             self.step(tokens)
+            if self.graph is not None and not self._captured_advance:
+                with self._ordered():
+                    self._advance()
+                self._move_on()
             last = self.next_tokens.tolist()
             for s, p in enumerate(prompts):
                 if self.host_positions[s] >= len(p):
