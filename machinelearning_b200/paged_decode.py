@@ -60,6 +60,8 @@ class PagedGemma3Decoder(Gemma3Decoder):
             for li in self.global_layers:
                 self.slot_weights[li] = torch.zeros(B, cfg.n_kv_heads, cap, dtype=torch.float32, device=dev)
                 self.slot_positions[li] = ints(B, cfg.n_kv_heads, cap) - 1
+            # where a step that stays at its position leaves its sums
+            self.unused_weights = torch.zeros(B, cfg.n_kv_heads, cap, dtype=torch.float32, device=dev)
         one, zero = torch.ones(B, device=dev), torch.zeros(B, device=dev)
         self.penalties = {"repetition": one, "presence": zero.clone(), "frequency": zero.clone()}
         self.bias_ids = self.bias_values = self.mask = self.mask_rows = None
@@ -113,7 +115,9 @@ class PagedGemma3Decoder(Gemma3Decoder):
         if not far:
             cache.attend(q, self.seen, self.inv_scale, window=self.window, out=out)
             return
-        cache.attend(q, self.global_seen, self.inv_scale, weights=self.slot_weights.get(li), out=out)
+        weights = self.slot_weights.get(li)
+        cache.attend(q, self.global_seen, self.inv_scale, weights=weights,
+                     weights_out=weights if weights is None or self._accumulates else self.unused_weights, out=out)
         if self.budget:  # the new slot's position (of idle sequences: what is there)
             at = self.slots.long().clamp(max=cache.capacity - 1)[:, None, None].expand(-1, cfg.n_kv_heads, 1)
             held = self.slot_positions[li]
@@ -125,6 +129,7 @@ class PagedGemma3Decoder(Gemma3Decoder):
         self.slots.add_(self.active)
 
     def _launch(self, advance: bool):
+        self._accumulates = advance
         # the step's token joins its sequence's history; idle rows keep what they hold
         at = self.positions.clamp(min=0, max=self.cfg.ctx - 1).long()[:, None]
         token = torch.where(self.active[:, None] > 0, self.tokens[:, None], self.history.gather(1, at))
@@ -141,31 +146,22 @@ class PagedGemma3Decoder(Gemma3Decoder):
             self._advance()
 
     def capture(self, advance: bool = True) -> None:
-        """As ``Gemma3Decoder.capture``; the direct launch before the capture leaves the
-        accumulated weights as they were."""
-        with self._ordered():
-            kept = {li: w.clone() for li, w in self.slot_weights.items()}
         super().capture(advance)
-        with self._ordered():
-            for li, w in kept.items():
-                self.slot_weights[li].copy_(w)
         self._captured_advance = advance
         self._captured_constraints = self.bias_ids, self.bias_values, self.mask, self.mask_rows  # read by replays
 
     def step(self, tokens=None, advance: bool = True) -> torch.Tensor:
         """Processed logits [batch][vocab] of one step of all started sequences (rows of idle
-        ones mean nothing); ``next_tokens`` holds their largest entries."""
+        ones mean nothing); ``next_tokens`` holds their largest entries. Without ``advance`` the
+        step can be repeated: positions and accumulated weights stay as they were."""
         if any(p >= self.cfg.ctx for p in self.host_positions):
             raise ValueError(f"a sequence is at the cache's capacity of {self.cfg.ctx} positions")
         if self.graph is not None:
             advance = self._captured_advance
         super().step(tokens, advance)
         if advance:
-            self._move_on()
+            self.host_positions = [p + (p >= 0) for p in self.host_positions]
         return self.processed
-
-    def _move_on(self) -> None:
-        self.host_positions = [p + (p >= 0) for p in self.host_positions]
 
     def evict(self) -> None:
         """Brings the global layers down to ``budget`` slots a sequence and kv head."""
@@ -194,6 +190,15 @@ class PagedGemma3Decoder(Gemma3Decoder):
             return [[] for _ in prompts]
         if any(p >= 0 for p in self.host_positions[len(prompts):]):
             raise ValueError("a sequence without a prompt is started: it would be fed tokens of nobody's")
+        graph = self.graph
+        if graph is not None and not self._captured_advance:
+            self.graph = None  # a step that stays where it is and adds no weights is not this loop's
+        try:
+            return self._generate(prompts, max_new_tokens, evict_every)
+        finally:
+            self.graph = graph
+
+    def _generate(self, prompts: list[list[int]], max_new_tokens: int, evict_every: int) -> list[list[int]]:
         for s, p in enumerate(prompts):
             self.start(s, len(p))
         out: list[list[int]] = [[] for _ in prompts]
@@ -205,10 +210,6 @@ class PagedGemma3Decoder(Gemma3Decoder):
                 if 0 <= self.host_positions[s] < len(p):
                     tokens[s] = p[self.host_positions[s]]
             self.step(tokens)
-            if self.graph is not None and not self._captured_advance:
-                with self._ordered():
-                    self._advance()
-                self._move_on()
             last = self.next_tokens.tolist()
             for s, p in enumerate(prompts):
                 if self.host_positions[s] >= len(p):

@@ -62,3 +62,45 @@ def test_generate_leaves_sequences_idle_and_refuses_first(oracle, torch):
         model.generate([[1, 2]], 2)
     assert model.host_positions == [-1, -1, 0]
     model.close()
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_a_repeated_step_adds_its_weights_once(oracle, torch, use_graph):
+    """step(advance=False) leaves the accumulated weights as they were, like the
+    position it stays at."""
+    from machinelearning_b200.paged_decode import PagedGemma3Decoder
+    cfg = small_config()
+    w = host_weights(oracle, cfg, seed=73)
+    got = []
+    for repeats in (0, 3):
+        model = PagedGemma3Decoder(cfg, w, batch=2, budget=4, recent=1)
+        for s in range(2):
+            model.start(s)
+        model.step([7, 8])
+        if use_graph and repeats:
+            model.capture(advance=False)
+        for _ in range(repeats):
+            model.step([9, 10], advance=False)
+        model.graph = None
+        model.step([9, 10])
+        got.append([model.slot_weights[li].clone() for li in model.global_layers] + [model.logits.clone()])
+        model.close()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_generate_evicts_alike_with_and_without_a_graph(oracle, torch):
+    """The weights that evictions go by are those of the steps taken, however they are launched."""
+    from machinelearning_b200.paged_decode import PagedGemma3Decoder
+    cfg = small_config()
+    w = host_weights(oracle, cfg, seed=76)
+    got = []
+    for graph in (None, True, False):
+        model = PagedGemma3Decoder(cfg, w, batch=2, budget=3, recent=1)
+        if graph is not None:
+            model.capture(advance=graph)
+        out = model.generate([[5, 9, 14], [600]], 8, evict_every=2)
+        got.append((out, [model.slot_positions[li].tolist() for li in model.global_layers]))
+        assert (model.graph is None) == (graph is None)
+        model.close()
+    assert got[0] == got[1] == got[2]
