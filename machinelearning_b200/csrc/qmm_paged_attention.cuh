@@ -293,6 +293,12 @@ __device__ __forceinline__ Found find(const AttendArgs& a, const Scratch& sc, in
     return f;
 }
 
+// A query's largest element is brought to 2^kRaise: f16 parts of smaller elements
+// keep their bits down to 2^-24 (from 1 on, one element of 2^15 among others of 1
+// left those 2^-10 of error).
+template <typename T>
+constexpr int kRaise = std::is_same_v<T, __half> ? 14 : 0;
+
 // Weights are relative to 2^m with m at most kSlack below the largest score so
 // far (in units of log 2): the sums are rescaled when it grows by more, not at
 // every new maximum (a few times a warp). f16 holds 2^-24 to 2^16: there the
@@ -427,7 +433,7 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
             }
             top = warp_max(top);
             int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-            e = max(-126, min(126, e));
+            e = max(-126, min(127, e - kRaise<T>));
             const float down = exp2f((float)-e);
             if (lane == 0) unit_s[j] = a.scale * kLog2e * exp2f((float)e);
 #pragma unroll

@@ -1,0 +1,93 @@
+"""Attention over a paged cache (machinelearning_b200/paged.py) where values are
+unlike each other or not finite, against the formula in 64 bits.
+
+With scores s and weights p = e^(s - max s) / sum of the same: a score of
+-infinity has weight 0 (all of them: the output is zero), one of +infinity
+or NaN makes its query head's output NaN; a weight above 0 times an infinite V is
+that infinity, 0 times it and the sum of both infinities are NaN. What a query
+head or a column of V holds changes no other head's or column's output.
+
+Tolerance of a finite output, u = 2^-24, stated before the first run: that of
+``test_paged_gpu.py``, of the sums without the terms that are not finite.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from test_paged_gpu import SPLIT, U, make_cache
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(4, 1, 256), (8, 2, 128), (24, 2, 64), (12, 1, 192)]
+LENGTHS = [5, 300, 20000, 17]  # the third is divided among CTAs
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available()
+    return torch
+
+
+def dense(cache, pages, b, n):
+    """f64 [kv heads][n][head_dim] of a sequence's first n slots."""
+    slots = np.arange(n)
+    table = cache.block_table[b].cpu().numpy()
+    t = pages[table[slots // cache.page_size], :, slots % cache.page_size].double().cpu().numpy()
+    return t.transpose(1, 0, 2)
+
+
+def put(cache, pages, b, slot, head, column, value):
+    pages[int(cache.block_table[b, slot // cache.page_size]), head, slot % cache.page_size, column] = value
+
+
+def reference(cache, q, lengths, scale, split):
+    """(out, tolerance) in 64 bits; q is finite."""
+    B, nq, hd = q.shape
+    g = nq // cache.n_kv_heads
+    q = q.double().cpu().numpy()
+    out, tol = np.zeros(q.shape), np.full(q.shape, 1e-30)
+    for b, n in enumerate(lengths):
+        k, v = dense(cache, cache.k, b, n), dense(cache, cache.v, b, n)
+        for h in range(nq):
+            kk, vv = k[h // g], v[h // g]
+            with np.errstate(invalid="ignore", over="ignore"):
+                s = (kk * q[b, h]).sum(-1) * scale
+                finite = np.isfinite(s)
+                if np.isneginf(s).all():
+                    continue
+                e = (np.abs(kk[finite]) @ np.abs(q[b, h])).max(initial=0.0) * scale * (split + hd * U)
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                out[b, h] = (p[:, None] * vv).sum(0)
+                tol[b, h] += p @ np.where(np.isfinite(vv), np.abs(vv), 0.0) * (2 * e + split + 2.0 ** -20)
+    return out, tol
+
+
+def check(got, ref, tol):
+    got = got.double().cpu().numpy()
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(ref))
+    off = ~np.isfinite(ref)
+    np.testing.assert_array_equal(got[off], ref[off])
+    worst = np.max(np.abs(got[~off] - ref[~off]) / tol[~off])
+    assert worst <= 1.0, f"off by {worst:.2f} times the tolerance"
+
+
+def problem(torch, dtype, nq, nkv, hd, seed):
+    cache = make_cache(torch, len(LENGTHS), max(LENGTHS), nkv, hd, dtype, 16, seed=seed)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(len(LENGTHS), nq, hd, generator=gen, device="cuda")
+    return cache, q, torch.tensor(LENGTHS, dtype=torch.int32, device="cuda"), hd ** -0.5
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nkv,hd", HEADS)
+@pytest.mark.parametrize("outlier", [2.0 ** 15, -3e4, 2.0 ** 7])
+def test_attend_queries_with_an_outlier(torch, dtype, nq, nkv, hd, outlier):
+    """One element of a query far above the others, where the keys are zero: the
+    scores are those of the others, to their own accuracy."""
+    cache, q, n, scale = problem(torch, dtype, nq, nkv, hd, 1)
+    q[..., 7] = outlier
+    cache.k[..., 7] = 0
+    check(cache.attend(q, n, scale), *reference(cache, q, LENGTHS, scale, SPLIT[dtype]))
