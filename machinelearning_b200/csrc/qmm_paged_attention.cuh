@@ -299,6 +299,23 @@ __device__ __forceinline__ Found find(const AttendArgs& a, const Scratch& sc, in
 template <typename T>
 constexpr int kRaise = std::is_same_v<T, __half> ? 14 : 0;
 
+// q . k in 32 bits from a K row in the ring (odd: an odd row of its step), where the
+// product by parts is not finite: a part of an infinity, or what an infinite key
+// meets, is NaN or has the other sign.
+template <typename T, int HD>
+__device__ __noinline__ float plain_dot(const uint8_t* k_row, int odd, const float* q) {
+    constexpr int kElems = 16 / (int)sizeof(T);
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < HD / kElems; ++c) {
+        const uint4 u = lds16(k_row + (c >> 3) * 128 + ((c & 7) ^ (odd * 4)) * 16);
+        const T* k = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) sum = fmaf(q[c * kElems + i], kv_to_f32<T>(k[i]), sum);
+    }
+    return sum;
+}
+
 // Weights are relative to 2^m with m at most kSlack below the largest score so
 // far (in units of log 2): the sums are rescaled when it grows by more, not at
 // every new maximum (a few times a warp). f16 holds 2^-24 to 2^16: there the
@@ -426,16 +443,19 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
         for (int j = warp; j < S::kHeads; j += W) {
             const float* q = a.q + b * a.ldq + (int64_t)(head0 + j) * HD;
             float x[HD / 32], top = 0.0f;
+            bool nan = false;
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
                 x[i] = j < nh ? q[lane + 32 * i] : 0.0f;
                 top = fmaxf(top, fabsf(x[i]));
+                nan = nan || x[i] != x[i];
             }
             top = warp_max(top);
+            nan = __any_sync(0xffffffffu, nan);
             int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
             e = max(-126, min(127, e - kRaise<T>));
             const float down = exp2f((float)-e);
-            if (lane == 0) unit_s[j] = a.scale * kLog2e * exp2f((float)e);
+            if (lane == 0) unit_s[j] = nan ? NAN : a.scale * kLog2e * exp2f((float)e);
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
                 const int d = lane + 32 * i, c = d / kElems, r = d % kElems;
@@ -539,11 +559,32 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                         }
                 }
             }
+            // lane (g, t) has the scores of heads g, g + 8 at slots 2 t, 2 t + 1 of every eight
+            float all = 0.0f;
 #pragma unroll
             for (int q = 0; q < SETS; ++q)
 #pragma unroll
-                for (int r = 0; r < kX; ++r) x[q][r] *= unit[q];
-            // lane (g, t) has the scores of heads g, g + 8 at slots 2 t, 2 t + 1 of every eight
+                for (int r = 0; r < kX; ++r) {
+                    x[q][r] *= unit[q];
+                    all += x[q][r];
+                }
+            if (!(fabsf(all) < INFINITY)) {  // each that is not finite, but for those of heads with NaN
+#pragma unroll 1
+                for (int n = 0; n < SETS * kX; ++n) {
+                    const int q = n / kX, r = n - q * kX;
+                    float u = 0.0f, old = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < SETS * kX; ++k)
+                        if (k == n) u = unit[k / kX], old = x[k / kX][k % kX];
+                    if (8 * q + g >= nh || u != u || fabsf(old) < INFINITY) continue;
+                    const uint8_t* row = ring + at * S::kUnit + (2 * t + (r & 1) + 8 * (r >> 1)) * S::kRow;
+                    const float s0 = plain_dot<T, HD>(row, r & 1, a.q + b * a.ldq + (int64_t)(head0 + 8 * q + g) * HD) *
+                                     (a.scale * kLog2e);
+#pragma unroll
+                    for (int k = 0; k < SETS * kX; ++k)
+                        if (k == n) x[k / kX][k % kX] = s0;
+                }
+            }
             const int slot0 = my_slot0 + i * (W * kSlots);
             bool whole = slot0 >= s.first && slot0 + kSlots <= s.n;
 #pragma unroll

@@ -91,3 +91,70 @@ def test_attend_queries_with_an_outlier(torch, dtype, nq, nkv, hd, outlier):
     q[..., 7] = outlier
     cache.k[..., 7] = 0
     check(cache.attend(q, n, scale), *reference(cache, q, LENGTHS, scale, SPLIT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nkv,hd", HEADS)
+def test_attend_infinite_keys(torch, dtype, nq, nkv, hd):
+    """Keys with an infinite element: weight 0 for the query heads on its far side,
+    NaN for those on its near side."""
+    cache, q, n, scale = problem(torch, dtype, nq, nkv, hd, 2)
+    q[..., 3] = 1.0   # exact in every type: its other parts are zero
+    q[:, 1::2, 3] = 0.7
+    for b, slots in enumerate(([0, 4], [16, 299], [0, 9000, 19999], [16])):
+        for i, slot in enumerate(slots):
+            put(cache, cache.k, b, slot, i % nkv, 3, float("-inf"))
+    ref = reference(cache, q, LENGTHS, scale, SPLIT[dtype])
+    assert np.isfinite(ref[0]).all()
+    check(cache.attend(q, n, scale), *ref)
+    q[0, 0, 3], q[2, nq - 1, 3] = -1.0, -0.3
+    put(cache, cache.k, 2, 12345, nkv - 1, 3, float("-inf"))
+    ref = reference(cache, q, LENGTHS, scale, SPLIT[dtype])
+    assert np.isnan(ref[0]).all(-1).sum() == 2
+    check(cache.attend(q, n, scale), *ref)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attend_weights_of_infinite_keys(torch, dtype):
+    """The slots' weights: 0 where the key is infinite; and all keys infinite: zeros."""
+    nq, nkv, hd = 8, 2, 128
+    cache, q, n, scale = problem(torch, dtype, nq, nkv, hd, 3)
+    q[..., 3] = 0.9
+    for slot in range(5):
+        put(cache, cache.k, 0, slot, 0, 3, float("-inf"))
+    put(cache, cache.k, 1, 77, 1, 3, float("-inf"))
+    w = torch.zeros(len(LENGTHS), nkv, cache.capacity, device="cuda")
+    out = cache.attend(q, n, scale, weights=w)
+    check(out, *reference(cache, q, LENGTHS, scale, SPLIT[dtype]))
+    assert not out[0, :4].any() and not w[0, 0].any() and out[0, 4:].any()
+    assert float(w[1, 1, 77]) == 0.0
+    np.testing.assert_allclose(w.sum(-1).cpu().numpy(), [[0, 4]] + [[4, 4]] * 3, rtol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attend_queries_that_are_not_finite(torch, dtype):
+    """NaN and infinite queries: NaN for their own head, and the others as without them."""
+    cache, q, n, scale = problem(torch, dtype, 24, 2, 64, 5)
+    ref, tol = reference(cache, q, LENGTHS, scale, SPLIT[dtype])
+    bad = q.clone()
+    bad[0, 1, 5], bad[1, 13, 0], bad[2, 23, 63] = float("nan"), float("inf"), float("-inf")
+    for b, h in ((0, 1), (1, 13), (2, 23)):
+        ref[b, h] = np.nan
+    check(cache.attend(bad, n, scale), ref, tol)
+
+
+def test_attend_f16_overflow_from_append(torch):
+    """A key beyond f16's range is an infinity in the cache: its slot has weight 0
+    for a query on its far side."""
+    cache = make_cache(torch, 1, 64, 1, 64, "f16", 16, seed=6)
+    qkv = torch.randn(1, 3 * 64, device="cuda")
+    qkv[0, 0], qkv[0, 64], qkv[0, 128 + 5] = 1.0, -7e4, 7e4
+    one = torch.ones(1, 32, device="cuda")
+    n = torch.tensor([33], dtype=torch.int32, device="cuda")
+    q = cache.append(qkv, torch.zeros_like(n), n - 1, one, torch.zeros_like(one), n_heads=1)
+    got = cache.attend(q, n - 32, 0.125)  # one other slot alone
+    assert torch.isfinite(got).all()
+    with_it = cache.attend(q, n, 0.125)
+    ref, tol = reference(cache, q, [33], 0.125, SPLIT["f16"])
+    assert np.isnan(ref[0, 0, 5]) and np.isfinite(ref[0, 0]).sum() == 63  # weight 0 times the infinite value
+    check(with_it, ref, tol)
