@@ -316,6 +316,44 @@ __device__ __noinline__ float plain_dot(const uint8_t* k_row, int odd, const flo
     return sum;
 }
 
+// Four columns of sum_t 2^(s_t - zero) v_t in 32 bits over slots [first, last), by a
+// warp, for columns of V that hold an infinity: a part of a weight that is zero or
+// below it makes NaN of one. f32 values that tf32 rounds to infinity count too: there
+// every slot is summed. k, v: the kv head's rows (v at the columns).
+template <typename T, int HD>
+__device__ __noinline__ float4 plain_values(const float* q, const T* k, const T* v, const int* table, int page_shift,
+                                            int n_pages, int64_t page_stride, int64_t slot_stride, int first, int last,
+                                            float scale, float zero) {
+    constexpr int kElems = 16 / (int)sizeof(T);
+    float c[4] = {0, 0, 0, 0};
+    for (int slot = first + (threadIdx.x & 31); slot < last; slot += 32) {
+        const int page = table[slot >> page_shift];
+        if (page < 0 || page >= n_pages) continue;
+        const int64_t row = page * page_stride + (slot & ((1 << page_shift) - 1)) * slot_stride;
+        float x[4];
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = kv_to_f32<T>(v[row + i]);
+            finite = finite && fabsf(x[i]) < INFINITY;
+        }
+        if (sizeof(T) == 2 && finite) continue;  // of no account beside the infinities
+        float s = 0.0f;
+#pragma unroll 1
+        for (int u = 0; u < HD / kElems; ++u) {
+            const uint4 bits = *reinterpret_cast<const uint4*>(k + row + u * kElems);
+            const T* e = reinterpret_cast<const T*>(&bits);
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) s = fmaf(q[u * kElems + i], kv_to_f32<T>(e[i]), s);
+        }
+        const float p = ex2(s * scale - zero);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (sizeof(T) == 4 || !(fabsf(x[i]) < INFINITY)) c[i] += p * x[i];
+    }
+    return make_float4(warp_sum(c[0]), warp_sum(c[1]), warp_sum(c[2]), warp_sum(c[3]));
+}
+
 // Weights are relative to 2^m with m at most kSlack below the largest score so
 // far (in units of log 2): the sums are rescaled when it grows by more, not at
 // every new maximum (a few times a warp). f16 holds 2^-24 to 2^16: there the
@@ -734,8 +772,10 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
         __syncthreads();
         const bool begins = tile == 0, ends = tile + count == s.tiles;
         const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-        for (int i = threadIdx.x; i < nh * (HD / 4); i += W * 32) {
-            const int j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
+        const int units = nh * (HD / 4);
+        for (int i0 = warp * 32; i0 < units; i0 += W * 32) {
+            const bool live = i0 + lane < units;
+            const int i = live ? i0 + lane : i0, j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; ++w) M = fmaxf(M, ml_s[w * S::kHeads + j].x);
@@ -752,6 +792,27 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                 o.z += p.z * f;
                 o.w += p.w * f;
             }
+            // columns that are not finite though the weights are (L is): one by one, by the whole warp
+            unsigned bad = __ballot_sync(0xffffffffu, live && L == L && !(fabsf((o.x + o.y) + (o.z + o.w)) < INFINITY));
+            while (bad) {
+                const int owner = __ffs(bad) - 1;
+                bad &= bad - 1;
+                const int first = max(s.first, (s.tile0 + tile) * kSlots);
+                const int last = min(s.n, (s.tile0 + tile + count) * kSlots);
+                const float4 v = plain_values<T, HD>(
+                    a.q + b * a.ldq + (int64_t)(head0 + __shfl_sync(0xffffffffu, j, owner)) * HD,
+                    static_cast<const T*>(a.kv.k) + kvh * a.kv.head_stride,
+                    static_cast<const T*>(a.kv.v) + kvh * a.kv.head_stride + __shfl_sync(0xffffffffu, d, owner), table,
+                    a.kv.page_shift, (int)a.kv.n_pages, a.kv.page_stride, a.kv.slot_stride, first, last,
+                    a.scale * kLog2e, __shfl_sync(0xffffffffu, M, owner) - kWeightBias<T>);
+                if (lane == owner) {
+                    if (!(fabsf(o.x) < INFINITY)) o.x = v.x;
+                    if (!(fabsf(o.y) < INFINITY)) o.y = v.y;
+                    if (!(fabsf(o.z) < INFINITY)) o.z = v.z;
+                    if (!(fabsf(o.w) < INFINITY)) o.w = v.w;
+                }
+            }
+            if (!live) continue;
             if (begins && ends) {
                 const float inv = L > 0.0f ? 1.0f / L : 0.0f;
                 *reinterpret_cast<float4*>(a.out + ((int64_t)b * a.nq + head0 + j) * HD + d) =

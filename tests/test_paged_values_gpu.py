@@ -158,3 +158,26 @@ def test_attend_f16_overflow_from_append(torch):
     ref, tol = reference(cache, q, [33], 0.125, SPLIT["f16"])
     assert np.isnan(ref[0, 0, 5]) and np.isfinite(ref[0, 0]).sum() == 63  # weight 0 times the infinite value
     check(with_it, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nkv,hd", HEADS)
+def test_attend_infinite_values(torch, dtype, nq, nkv, hd):
+    """Values with infinities and NaN: their own columns only, of the kv head's query heads."""
+    cache, q, n, scale = problem(torch, dtype, nq, nkv, hd, 4)
+    inf, nan = float("inf"), float("nan")
+    for b, slots in enumerate(([0, 3], [31, 150], [5, 19990], [8, 16])):
+        put(cache, cache.v, b, slots[0], 0, 0, inf)
+        put(cache, cache.v, b, slots[1], 0, 0, inf)
+        put(cache, cache.v, b, slots[0], 0, 9, -inf)
+        put(cache, cache.v, b, slots[0], nkv - 1, hd - 1, inf)
+        put(cache, cache.v, b, slots[1], nkv - 1, hd - 1, -inf)  # both: NaN
+        put(cache, cache.v, b, slots[1], nkv - 1, 40, nan)
+    q[..., 3] = 1.0
+    put(cache, cache.k, 1, 10, 0, 3, -inf)  # weight 0 of an infinity: NaN
+    put(cache, cache.v, 1, 10, 0, 33, inf)
+    ref = reference(cache, q, LENGTHS, scale, SPLIT[dtype])
+    g = nq // nkv
+    assert (ref[0][:, :g, 0] == inf).all() and (ref[0][:, :g, 9] == -inf).all()
+    assert np.isnan(ref[0][:, -g:, hd - 1]).all() and np.isnan(ref[0][1, :g, 33]).all()
+    check(cache.attend(q, n, scale), *ref)
