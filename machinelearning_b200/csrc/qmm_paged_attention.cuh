@@ -299,61 +299,6 @@ __device__ __forceinline__ Found find(const AttendArgs& a, const Scratch& sc, in
 template <typename T>
 constexpr int kRaise = std::is_same_v<T, __half> ? 14 : 0;
 
-// q . k in 32 bits from a K row in the ring (odd: an odd row of its step), where the
-// product by parts is not finite: a part of an infinity, or what an infinite key
-// meets, is NaN or has the other sign.
-template <typename T, int HD>
-__device__ __noinline__ float plain_dot(const uint8_t* k_row, int odd, const float* q) {
-    constexpr int kElems = 16 / (int)sizeof(T);
-    float sum = 0.0f;
-#pragma unroll 1
-    for (int c = 0; c < HD / kElems; ++c) {
-        const uint4 u = lds16(k_row + (c >> 3) * 128 + ((c & 7) ^ (odd * 4)) * 16);
-        const T* k = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int i = 0; i < kElems; ++i) sum = fmaf(q[c * kElems + i], kv_to_f32<T>(k[i]), sum);
-    }
-    return sum;
-}
-
-// Four columns of sum_t 2^(s_t - zero) v_t in 32 bits over slots [first, last), by a
-// warp, for columns of V that hold an infinity: a part of a weight that is zero or
-// below it makes NaN of one. f32 values that tf32 rounds to infinity count too: there
-// every slot is summed. k, v: the kv head's rows (v at the columns).
-template <typename T, int HD>
-__device__ __noinline__ float4 plain_values(const float* q, const T* k, const T* v, const int* table, int page_shift,
-                                            int n_pages, int64_t page_stride, int64_t slot_stride, int first, int last,
-                                            float scale, float zero) {
-    constexpr int kElems = 16 / (int)sizeof(T);
-    float c[4] = {0, 0, 0, 0};
-    for (int slot = first + (threadIdx.x & 31); slot < last; slot += 32) {
-        const int page = table[slot >> page_shift];
-        if (page < 0 || page >= n_pages) continue;
-        const int64_t row = page * page_stride + (slot & ((1 << page_shift) - 1)) * slot_stride;
-        float x[4];
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = kv_to_f32<T>(v[row + i]);
-            finite = finite && fabsf(x[i]) < INFINITY;
-        }
-        if (sizeof(T) == 2 && finite) continue;  // of no account beside the infinities
-        float s = 0.0f;
-#pragma unroll 1
-        for (int u = 0; u < HD / kElems; ++u) {
-            const uint4 bits = *reinterpret_cast<const uint4*>(k + row + u * kElems);
-            const T* e = reinterpret_cast<const T*>(&bits);
-#pragma unroll
-            for (int i = 0; i < kElems; ++i) s = fmaf(q[u * kElems + i], kv_to_f32<T>(e[i]), s);
-        }
-        const float p = ex2(s * scale - zero);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (sizeof(T) == 4 || !(fabsf(x[i]) < INFINITY)) c[i] += p * x[i];
-    }
-    return make_float4(warp_sum(c[0]), warp_sum(c[1]), warp_sum(c[2]), warp_sum(c[3]));
-}
-
 // Weights are relative to 2^m with m at most kSlack below the largest score so
 // far (in units of log 2): the sums are rescaled when it grows by more, not at
 // every new maximum (a few times a warp). f16 holds 2^-24 to 2^16: there the
@@ -362,6 +307,82 @@ template <typename T>
 constexpr float kWeightBias = std::is_same_v<T, __half> ? 14.0f : 0.0f;
 template <typename T>
 constexpr float kSlack = std::is_same_v<T, __half> ? 1.0f : 8.0f;
+
+// A piece of one query head in 32 bits, by a warp, where the products by parts are
+// not finite: what an infinity in K or V meets, a part of zero or of the other sign,
+// makes NaN of it. Lanes sum the four columns at v_cols of their own; known: M and L
+// are, and only the columns asked for. scores null, or the head's row of them. For
+// data with infinities only: 131071 slots of 64/8 heads of 128, bf16, with some in
+// every page take 3.4 ms instead of 93 us.
+template <typename T>
+struct PlainPiece {
+    const float* q;
+    const T* k;  // the kv head's rows
+    const T* v_cols;
+    const int* table;
+    int64_t page_stride, slot_stride;
+    int page_shift, n_pages, first, last;  // slots [first, last)
+    float scale;                           // log2(e) in it
+    float* scores;
+};
+template <typename T, int HD>
+__device__ __noinline__ float4 plain_piece(PlainPiece<T> a, bool known, float& M, float& L) {
+    constexpr int kElems = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    auto row_of = [&](int slot) -> int64_t {
+        const int page = slot < a.last ? a.table[slot >> a.page_shift] : -1;
+        if (page < 0 || page >= a.n_pages) return -1;
+        return page * a.page_stride + (slot & ((1 << a.page_shift) - 1)) * a.slot_stride;
+    };
+    auto score = [&](int64_t row) {
+        if (row < 0) return -INFINITY;
+        float s = 0.0f;
+#pragma unroll 1
+        for (int u = 0; u < HD / kElems; ++u) {
+            const uint4 bits = *reinterpret_cast<const uint4*>(a.k + row + u * kElems);
+            const T* e = reinterpret_cast<const T*>(&bits);
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) s = fmaf(a.q[u * kElems + i], kv_to_f32<T>(e[i]), s);
+        }
+        return s * a.scale;
+    };
+    if (!known) {
+        bool nan = false;
+        for (int d = lane; d < HD; d += 32) nan = nan || a.q[d] != a.q[d];
+        if (__any_sync(0xffffffffu, nan)) return make_float4(NAN, NAN, NAN, NAN);  // and L is as it was
+        M = -INFINITY;
+        nan = false;
+        for (int slot = a.first + lane; slot < a.last; slot += 32) {
+            const float s = score(row_of(slot));
+            if (a.scores) a.scores[slot] = s;
+            nan = nan || s != s;
+            M = fmaxf(M, s);
+        }
+        M = warp_max(M);
+        if (__any_sync(0xffffffffu, nan)) return make_float4(NAN, NAN, NAN, NAN);
+    }
+    const float zero = M == -INFINITY ? 0.0f : M - kWeightBias<T>;
+    float sum = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int s0 = a.first; s0 < a.last; s0 += 32) {
+        const int64_t mine = row_of(s0 + lane);
+        const float p_mine = ex2(score(mine) - zero);
+        sum += p_mine;
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const int64_t row = __shfl_sync(0xffffffffu, mine, i);
+            const float p = __shfl_sync(0xffffffffu, p_mine, i);
+            if (row < 0) continue;
+            const T* v = a.v_cols + row;
+            o.x += p * kv_to_f32<T>(v[0]);
+            o.y += p * kv_to_f32<T>(v[1]);
+            o.z += p * kv_to_f32<T>(v[2]);
+            o.w += p * kv_to_f32<T>(v[3]);
+        }
+    }
+    if (!known) L = warp_sum(sum);
+    return o;
+}
 
 // Every warp takes each kWarps-th step of the piece, and runs on its own until
 // the piece ends. The lane layout of the matrix instructions is met without a
@@ -481,19 +502,16 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
         for (int j = warp; j < S::kHeads; j += W) {
             const float* q = a.q + b * a.ldq + (int64_t)(head0 + j) * HD;
             float x[HD / 32], top = 0.0f;
-            bool nan = false;
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
                 x[i] = j < nh ? q[lane + 32 * i] : 0.0f;
                 top = fmaxf(top, fabsf(x[i]));
-                nan = nan || x[i] != x[i];
             }
             top = warp_max(top);
-            nan = __any_sync(0xffffffffu, nan);
             int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
             e = max(-126, min(127, e - kRaise<T>));
             const float down = exp2f((float)-e);
-            if (lane == 0) unit_s[j] = nan ? NAN : a.scale * kLog2e * exp2f((float)e);
+            if (lane == 0) unit_s[j] = a.scale * kLog2e * exp2f((float)e);
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
                 const int d = lane + 32 * i, c = d / kElems, r = d % kElems;
@@ -597,32 +615,11 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                         }
                 }
             }
-            // lane (g, t) has the scores of heads g, g + 8 at slots 2 t, 2 t + 1 of every eight
-            float all = 0.0f;
 #pragma unroll
             for (int q = 0; q < SETS; ++q)
 #pragma unroll
-                for (int r = 0; r < kX; ++r) {
-                    x[q][r] *= unit[q];
-                    all += x[q][r];
-                }
-            if (!(fabsf(all) < INFINITY)) {  // each that is not finite, but for those of heads with NaN
-#pragma unroll 1
-                for (int n = 0; n < SETS * kX; ++n) {
-                    const int q = n / kX, r = n - q * kX;
-                    float u = 0.0f, old = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < SETS * kX; ++k)
-                        if (k == n) u = unit[k / kX], old = x[k / kX][k % kX];
-                    if (8 * q + g >= nh || u != u || fabsf(old) < INFINITY) continue;
-                    const uint8_t* row = ring + at * S::kUnit + (2 * t + (r & 1) + 8 * (r >> 1)) * S::kRow;
-                    const float s0 = plain_dot<T, HD>(row, r & 1, a.q + b * a.ldq + (int64_t)(head0 + 8 * q + g) * HD) *
-                                     (a.scale * kLog2e);
-#pragma unroll
-                    for (int k = 0; k < SETS * kX; ++k)
-                        if (k == n) x[k / kX][k % kX] = s0;
-                }
-            }
+                for (int r = 0; r < kX; ++r) x[q][r] *= unit[q];
+            // lane (g, t) has the scores of heads g, g + 8 at slots 2 t, 2 t + 1 of every eight
             const int slot0 = my_slot0 + i * (W * kSlots);
             bool whole = slot0 >= s.first && slot0 + kSlots <= s.n;
 #pragma unroll
@@ -772,55 +769,84 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
         __syncthreads();
         const bool begins = tile == 0, ends = tile + count == s.tiles;
         const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-        const int units = nh * (HD / 4);
-        for (int i0 = warp * 32; i0 < units; i0 += W * 32) {
-            const bool live = i0 + lane < units;
-            const int i = live ? i0 + lane : i0, j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
-            float M = -INFINITY, L = 0.0f;
+        struct Sums {
+            float M, L;
+            float4 o;
+        };
+        auto sums_of = [&](int j, int d) {  // of the warps, at four columns of a head
+            Sums r = {-INFINITY, 0.0f, make_float4(0, 0, 0, 0)};
 #pragma unroll
-            for (int w = 0; w < W; ++w) M = fmaxf(M, ml_s[w * S::kHeads + j].x);
-            float4 o = make_float4(0, 0, 0, 0);
+            for (int w = 0; w < W; ++w) r.M = fmaxf(r.M, ml_s[w * S::kHeads + j].x);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 const float2 ml = ml_s[w * S::kHeads + j];
-                const float f = piece_factor(ml.x, M);
-                L += ml.y * f;
+                const float f = piece_factor(ml.x, r.M);
+                r.L += ml.y * f;
                 const float4 p = *reinterpret_cast<const float4*>(
                     reinterpret_cast<const float*>(smem + w * S::kUnits * S::kUnit) + j * S::kAccRow + d);
-                o.x += p.x * f;
-                o.y += p.y * f;
-                o.z += p.z * f;
-                o.w += p.w * f;
+                r.o.x += p.x * f;
+                r.o.y += p.y * f;
+                r.o.z += p.z * f;
+                r.o.w += p.w * f;
             }
-            // columns that are not finite though the weights are (L is): one by one, by the whole warp
-            unsigned bad = __ballot_sync(0xffffffffu, live && L == L && !(fabsf((o.x + o.y) + (o.z + o.w)) < INFINITY));
-            while (bad) {
-                const int owner = __ffs(bad) - 1;
-                bad &= bad - 1;
-                const int first = max(s.first, (s.tile0 + tile) * kSlots);
-                const int last = min(s.n, (s.tile0 + tile + count) * kSlots);
-                const float4 v = plain_values<T, HD>(
-                    a.q + b * a.ldq + (int64_t)(head0 + __shfl_sync(0xffffffffu, j, owner)) * HD,
-                    static_cast<const T*>(a.kv.k) + kvh * a.kv.head_stride,
-                    static_cast<const T*>(a.kv.v) + kvh * a.kv.head_stride + __shfl_sync(0xffffffffu, d, owner), table,
-                    a.kv.page_shift, (int)a.kv.n_pages, a.kv.page_stride, a.kv.slot_stride, first, last,
-                    a.scale * kLog2e, __shfl_sync(0xffffffffu, M, owner) - kWeightBias<T>);
-                if (lane == owner) {
-                    if (!(fabsf(o.x) < INFINITY)) o.x = v.x;
-                    if (!(fabsf(o.y) < INFINITY)) o.y = v.y;
-                    if (!(fabsf(o.z) < INFINITY)) o.z = v.z;
-                    if (!(fabsf(o.w) < INFINITY)) o.w = v.w;
-                }
-            }
-            if (!live) continue;
+            return r;
+        };
+        auto store = [&](int j, int d, const Sums& r) {
             if (begins && ends) {
-                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+                const float inv = r.L > 0.0f ? 1.0f / r.L : 0.0f;
                 *reinterpret_cast<float4*>(a.out + ((int64_t)b * a.nq + head0 + j) * HD + d) =
-                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-                if (sc.whole && d == 0) sc.whole[(int64_t)b * a.nq + head0 + j] = make_float2(M, L);
+                    make_float4(r.o.x * inv, r.o.y * inv, r.o.z * inv, r.o.w * inv);
+                if (sc.whole && d == 0) sc.whole[(int64_t)b * a.nq + head0 + j] = make_float2(r.M, r.L);
             } else {
-                *reinterpret_cast<float4*>(sc.acc + ((int64_t)slot * S::kHeads + j) * HD + d) = o;
-                if (d == 0) sc.ml[slot * S::kHeads + j] = make_float2(M, L);
+                *reinterpret_cast<float4*>(sc.acc + ((int64_t)slot * S::kHeads + j) * HD + d) = r.o;
+                if (d == 0) sc.ml[slot * S::kHeads + j] = make_float2(r.M, r.L);
+            }
+        };
+        auto finite = [](const Sums& r) {
+            return r.L < INFINITY && fabsf((r.o.x + r.o.y) + (r.o.z + r.o.w)) < INFINITY;
+        };
+        bool bad = false;
+        for (int i = threadIdx.x; i < nh * (HD / 4); i += W * 32) {
+            const int j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
+            const Sums r = sums_of(j, d);
+            bad = bad || !finite(r);
+            store(j, d, r);
+        }
+        if (__any_sync(0xffffffffu, bad)) {  // the warp takes its own columns again, head by head
+            for (int i0 = warp * 32; i0 < nh * (HD / 4); i0 += W * 32) {
+                const int i = min(i0 + lane, nh * (HD / 4) - 1), j = i / (HD / 4), d = 4 * (i - j * (HD / 4));
+                Sums r = sums_of(j, d);
+                unsigned left = __ballot_sync(0xffffffffu, !finite(r));
+                while (left) {
+                    const int head = __shfl_sync(0xffffffffu, j, __ffs(left) - 1);
+                    left &= ~__ballot_sync(0xffffffffu, j == head);
+                    PlainPiece<T> plain;
+                    plain.q = a.q + b * a.ldq + (int64_t)(head0 + head) * HD;
+                    plain.k = static_cast<const T*>(a.kv.k) + kvh * a.kv.head_stride;
+                    plain.v_cols = static_cast<const T*>(a.kv.v) + kvh * a.kv.head_stride + d;
+                    plain.table = table;
+                    plain.page_stride = a.kv.page_stride;
+                    plain.slot_stride = a.kv.slot_stride;
+                    plain.page_shift = a.kv.page_shift;
+                    plain.n_pages = (int)a.kv.n_pages;
+                    plain.first = max(s.first, (s.tile0 + tile) * kSlots);
+                    plain.last = min(s.n, (s.tile0 + tile + count) * kSlots);
+                    plain.scale = a.scale * kLog2e;
+                    plain.scores =
+                        sc.scores ? sc.scores + ((int64_t)b * a.nq + head0 + head) * a.kv.capacity() : nullptr;
+                    const int owner = __ffs(__ballot_sync(0xffffffffu, j == head)) - 1;
+                    float M = __shfl_sync(0xffffffffu, r.M, owner), L = __shfl_sync(0xffffffffu, r.L, owner);
+                    const bool known = L < INFINITY;
+                    const float4 v = plain_piece<T, HD>(plain, known, M, L);
+                    if (j != head) continue;
+                    if (!known || !(fabsf(r.o.x) < INFINITY)) r.o.x = v.x;
+                    if (!known || !(fabsf(r.o.y) < INFINITY)) r.o.y = v.y;
+                    if (!known || !(fabsf(r.o.z) < INFINITY)) r.o.z = v.z;
+                    if (!known || !(fabsf(r.o.w) < INFINITY)) r.o.w = v.w;
+                    r.M = M;
+                    r.L = L;
+                    store(j, d, r);
+                }
             }
         }
         base += s.tiles + S::kSetup;
