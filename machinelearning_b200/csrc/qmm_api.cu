@@ -1049,7 +1049,9 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // The kernels' view of a caller's cache description.
 int paged_view(const qmm_paged_kv* in, PagedKv* out) {
-    if (!in || !in->k_dev || !in->v_dev || !in->table_dev) return fail(QMM_ERR_INVALID_INPUT, "null pointer");
+    // no sequences: nothing is read from or written to the cache
+    if (!in || (in->n_seqs != 0 && (!in->k_dev || !in->v_dev || !in->table_dev)))
+        return fail(QMM_ERR_INVALID_INPUT, "null pointer");
     const int size = kv_type_size(in->dtype);
     if (!size) return fail(QMM_ERR_DTYPE_MISMATCH, "cache type is not f32, f16 or bf16");
     if (in->head_dim <= 0 || in->head_dim % 64 || in->head_dim > 256)

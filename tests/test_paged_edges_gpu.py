@@ -1,0 +1,34 @@
+"""Caches and arguments at the edge of what the Python forms take (machinelearning_b200/paged.py)."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available()
+    return torch
+
+
+@pytest.mark.parametrize("pages", [0, 4])
+def test_empty_batches(torch, pages):
+    from machinelearning_b200.paged import PagedKVCache
+    k = torch.randn(pages, 2, 16, 64, device="cuda")
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = PagedKVCache(k, k.clone(), ints(0, 3))
+    q = torch.empty(0, 4, 64, device="cuda")
+    w = torch.empty(0, 2, 48, device="cuda")
+    assert cache.attend(q, ints(0), 1.0).shape == (0, 4, 64)
+    assert cache.attend(q, ints(0), 1.0, weights=w).shape == (0, 4, 64)
+    assert [t.shape for t in cache.evict(ints(0), w, ints(0, 2, 48), ints(0), 8, 2)] == [(0,), (0, 2, 48), (0, 2, 48)]
+    one = torch.ones(4, 32, device="cuda")
+    assert cache.append(torch.empty(0, 8 * 64, device="cuda"), ints(0), ints(0), one, one, n_heads=4).shape == (0, 4, 64)
+    # tokens of sequences that are gone: their queries, and nothing stored
+    qkv = torch.randn(3, 8 * 64, device="cuda")
+    before = k.clone()
+    got = cache.append(qkv, ints(3), ints(3), one, torch.zeros_like(one), n_heads=4, seqs=ints(3))
+    assert torch.equal(got.view(3, -1), qkv[:, :4 * 64]) and torch.equal(cache.k, before)
+    assert PagedKVCache.allocate(0, 48, 2, 64).attend(q, ints(0), 1.0).shape == (0, 4, 64)
