@@ -40,7 +40,7 @@ class PagedKVCache:
     be strided views (one pool for all layers, say) with contiguous rows."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor):
-        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
+        if k.dim() != 4 or k.shape != v.shape or self._strides(k) != self._strides(v):
             raise _mismatch("k and v: [pages][kv heads][slots][head_dim], of equal shape and strides")
         if k.dtype not in KV_DTYPES or v.dtype != k.dtype:
             raise _lib.DTypeMismatch(_lib.ERR_DTYPE_MISMATCH, f"cache types {k.dtype}, {v.dtype}")
@@ -48,7 +48,7 @@ class PagedKVCache:
             raise _mismatch("block_table: int32 [sequences][pages]")
         if not k.is_cuda or v.device != k.device or block_table.device != k.device:
             raise ValueError("k, v and block_table have to be on one GPU")
-        if k.stride(3) != 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        if k.stride(3) != 1 or v.stride(3) != 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
             raise _mismatch("rows of the cache and of the block table have to be contiguous")
         self.k, self.v, self.block_table = k, v, block_table
         self.device = k.device
@@ -56,15 +56,18 @@ class PagedKVCache:
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.n_seqs, self.max_pages = block_table.shape
         self.capacity = self.max_pages * self.page_size  # slots of one sequence
-        # a dimension of size one has any stride
-        stride = [max(s, self.head_dim) if n == 1 else s for n, s in zip(k.shape[:3], k.stride()[:3])]
         self._desc = _lib.PagedKv(k.data_ptr(), v.data_ptr(), KV_DTYPES[k.dtype], self.n_kv_heads, self.head_dim,
-                                  self.page_size, self.n_pages, *stride, block_table.data_ptr(), self.n_seqs,
+                                  self.page_size, self.n_pages, *self._strides(k), block_table.data_ptr(), self.n_seqs,
                                   self.max_pages, block_table.stride(0) if self.n_seqs > 1 else self.max_pages)
         self._ref = ctypes.byref(self._desc)
         self._lib = _lib.lib()
         self._seqs_shape = (self.n_seqs,)
         self._slots_shape = (self.n_seqs, self.n_kv_heads, self.capacity)
+
+    @staticmethod
+    def _strides(t: torch.Tensor) -> list[int]:
+        """Of pages, heads and slots; a dimension of size one has any stride."""
+        return [t.shape[3] if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
 
     @classmethod
     def allocate(cls, n_seqs: int, capacity: int, n_kv_heads: int, head_dim: int, page_size: int = 16,

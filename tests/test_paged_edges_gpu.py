@@ -32,3 +32,24 @@ def test_empty_batches(torch, pages):
     got = cache.append(qkv, ints(3), ints(3), one, torch.zeros_like(one), n_heads=4, seqs=ints(3))
     assert torch.equal(got.view(3, -1), qkv[:, :4 * 64]) and torch.equal(cache.k, before)
     assert PagedKVCache.allocate(0, 48, 2, 64).attend(q, ints(0), 1.0).shape == (0, 4, 64)
+
+
+def test_strides_of_dimensions_of_size_one_do_not_matter(torch):
+    """K and V from differently laid out pools that are alike but for such a stride, or
+    whose stride there is no multiple of 16 bytes."""
+    from machinelearning_b200.paged import PagedKVCache
+    n = torch.tensor([40], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    k = torch.randn(3, 16, 1, 64, device="cuda").transpose(1, 2)  # [slot][head] pages
+    v = torch.randn(3, 1, 16, 64, device="cuda")                  # [head][slot] pages
+    assert k.shape == v.shape and k.stride() != v.stride()
+    q = torch.randn(1, 4, 64, device="cuda")
+    want = PagedKVCache(k.contiguous(), v, table).attend(q, n, 0.1)
+    assert torch.equal(PagedKVCache(k, v, table).attend(q, n, 0.1), want)
+    odd = v.as_strided(v.shape, (1024, 1023, 64, 1))
+    assert torch.equal(PagedKVCache(k, odd, table).attend(q, n, 0.1), want)
+    assert torch.equal(PagedKVCache(odd, odd, table).attend(q, n, 0.1), PagedKVCache(v, v, table).attend(q, n, 0.1))
+    one_page = v[:1].as_strided((1, 1, 16, 64), (1, 1, 64, 1))
+    table0 = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    assert torch.equal(PagedKVCache(one_page, one_page, table0).attend(q, n, 0.1),
+                       PagedKVCache(v[:1], v[:1], table0).attend(q, n, 0.1))
