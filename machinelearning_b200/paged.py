@@ -198,6 +198,10 @@ class PagedKVCache:
         what ``attend`` (with ``weights``) and ``evict`` (``budget`` > 0) of this cache
         need; call it before capturing them in a CUDA graph."""
         need = self._lib.qmm_paged_attention_workspace_size(self._ref, int(n_heads), int(weights))
+        if not need:
+            raise _mismatch(f"{n_heads} query heads on {self.n_kv_heads} kv heads, or a cache that attend refuses")
+        if budget < 0:
+            raise ValueError(f"budget {budget}")
         if budget:
             need = max(need, self._lib.qmm_paged_evict_workspace_size(self._ref, int(budget)))
         stream = torch.cuda.current_stream(self.device) if stream is None else stream

@@ -53,3 +53,15 @@ def test_strides_of_dimensions_of_size_one_do_not_matter(torch):
     table0 = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
     assert torch.equal(PagedKVCache(one_page, one_page, table0).attend(q, n, 0.1),
                        PagedKVCache(v[:1], v[:1], table0).attend(q, n, 0.1))
+
+
+def test_reserve_refuses_what_attend_would(torch):
+    from machinelearning_b200 import _lib
+    from machinelearning_b200.paged import PagedKVCache
+    cache = PagedKVCache.allocate(1, 64, 2, 64)
+    cache.reserve(4, weights=True, budget=10)
+    for heads in (3, 0, -2):
+        with pytest.raises(_lib.ShapeMismatch):
+            cache.reserve(heads)
+    with pytest.raises(ValueError):
+        cache.reserve(4, budget=-1)
