@@ -409,7 +409,8 @@ QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, 
  * mask_rows_dev[i] of mask_dev [n_masks][ceil(vocab / 32)] is clear (a state
  * outside [0, n_masks): no mask; mask_rows_dev null: state i). Null tokens_dev,
  * bias_ids_dev or mask_dev: that step is left out; null prompt_lengths_dev: no
- * prompt; null penalties: 1, 0, 0. Ids outside [0, vocab) are ignored. */
+ * prompt; null penalties: 1, 0, 0. Ids outside [0, vocab) are ignored. max_tokens
+ * is below 2^30. */
 #define QMM_MAX_BIAS 1024
 QMM_API int qmm_process_logits_dev(const float* logits_dev, size_t ld, size_t rows, size_t vocab,
                                    const int* tokens_dev, size_t ld_tokens, size_t max_tokens,

@@ -1244,9 +1244,10 @@ QMM_API int qmm_process_logits_dev(const float* logits_dev, size_t ld, size_t ro
         if (!logits_dev || !out_dev || (tokens_dev && !token_lengths_dev) || (bias_ids_dev && !bias_values_dev))
             return fail(QMM_ERR_INVALID_INPUT, "null pointer");
         if (rows > 65535 || vocab > (size_t)INT32_MAX - 65536 || ld < vocab || ld_out < vocab || n_bias > kMaxBias ||
-            n_masks > (size_t)INT32_MAX || max_tokens > (size_t)INT32_MAX || (tokens_dev && ld_tokens < max_tokens))
+            n_masks > (size_t)INT32_MAX || max_tokens > (size_t)kMaxHistory || (tokens_dev && ld_tokens < max_tokens))
             return fail(QMM_ERR_SHAPE_MISMATCH,
-                        "rows (at most 65535), vocabulary, row stride, history, biases (at most 1024) out of range");
+                        "rows (at most 65535), vocabulary, row stride, history (below 2^30), biases (at most 1024) out of "
+                        "range");
         if (mask_dev && !mask_rows_dev && n_masks < rows)
             return fail(QMM_ERR_SHAPE_MISMATCH, "fewer masks than rows");
         if (logits_dev == out_dev && ld != ld_out)

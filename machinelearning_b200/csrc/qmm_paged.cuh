@@ -126,6 +126,7 @@ struct LogitsArgs {
     int64_t ld_out;
 };
 constexpr int kMaxBias = 1024;
+constexpr int kMaxHistory = (1 << 30) - 1;  // a token's count and two flags share a word
 cudaError_t launch_process_logits(const LogitsArgs& a, cudaStream_t st);
 
 }  // namespace qmm

@@ -19,3 +19,11 @@ def test_no_sequences_need_no_memory(qlib, change):
     assert qlib.qmm_paged_attention_workspace_size(kv, 4, 1) > 0
     one = desc(n_seqs=1, **change)
     assert attend(qlib, ctypes.byref(one)) == INVALID and append(qlib, ctypes.byref(one)) == INVALID
+
+
+def test_histories_whose_counts_would_not_fit(qlib):
+    """A count of 2^30 would run into the flags beside it."""
+    from test_paged import SHAPE, logits
+    for n in (1 << 30, (1 << 31) - 1):
+        assert logits(qlib, tokens=P, lens=P, ld_tokens=n, n=n) == SHAPE
+        assert b"history" in qlib.qmm_last_error_message()
