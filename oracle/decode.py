@@ -50,9 +50,10 @@ def rope(x, cos, sin):
     return np.concatenate([x1 * cos - x2 * sin, x1 * sin + x2 * cos], axis=-1).astype(F)
 
 
-def decode_step(cfg, w, tokens, pos: int, k_cache, v_cache):
+def decode_step(cfg, w, tokens, pos: int, k_cache, v_cache, window: int = 0):
     """Logits [B][vocab] of one decode step at position ``pos``; k_cache /
-    v_cache [layers][B][n_kv][ctx][head_dim] are updated in place.
+    v_cache [layers][B][n_kv][ctx][head_dim] are updated in place. ``window`` > 0:
+    the local layers see the last ``window`` positions only.
 
     ``cfg``: hidden, n_layers, n_heads, n_kv_heads, head_dim, ffn, vocab, ctx,
     eps, offset, rope_local, rope_global, pattern, query_pre_attn_scalar,
@@ -74,7 +75,9 @@ def decode_step(cfg, w, tokens, pos: int, k_cache, v_cache):
         q = rmsnorm(qkv[:, :nq], lw["q_norm"], cfg.offset, cfg.eps)
         k = rmsnorm(qkv[:, nq:nq + nkv], lw["k_norm"], cfg.offset, cfg.eps)
         v = qkv[:, nq + nkv:]
-        cos, sin = tables[cfg.rope_global if (li + 1) % cfg.pattern == 0 else cfg.rope_local]
+        far = (li + 1) % cfg.pattern == 0
+        first = max(0, pos + 1 - window) if window and not far else 0
+        cos, sin = tables[cfg.rope_global if far else cfg.rope_local]
         q = rope(q, cos[pos], sin[pos])
         k = rope(k, cos[pos], sin[pos])
         k_cache[li][:, :, pos] = k
@@ -83,10 +86,10 @@ def decode_step(cfg, w, tokens, pos: int, k_cache, v_cache):
         for b in range(B):
             for hh in range(nq):
                 kv = hh // (nq // nkv)
-                s = (k_cache[li][b, kv, :pos + 1] @ q[b, hh]).astype(F) * inv_scale
+                s = (k_cache[li][b, kv, first:pos + 1] @ q[b, hh]).astype(F) * inv_scale
                 p = np.exp(s - s.max()).astype(F)
                 p = (p / p.sum(dtype=F)).astype(F)
-                ctx[b, hh] = p @ v_cache[li][b, kv, :pos + 1]
+                ctx[b, hh] = p @ v_cache[li][b, kv, first:pos + 1]
         o = matmul_f32_q4(ctx.ravel(), lw["o"], B, nq * hd, H).reshape(B, H)
         x = (x + rmsnorm(o, lw["post_attn_norm"], cfg.offset, cfg.eps)).astype(F)
         h2 = rmsnorm(x, lw["ffn_norm"], cfg.offset, cfg.eps)

@@ -2,6 +2,7 @@
 step and leaves behind."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 from test_decode_gpu import host_weights, small_config
@@ -104,3 +105,55 @@ def test_generate_evicts_alike_with_and_without_a_graph(oracle, torch):
         assert (model.graph is None) == (graph is None)
         model.close()
     assert got[0] == got[1] == got[2]
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_windows_of_the_local_layers_match_the_oracle(oracle, torch, use_graph):
+    """Logits at the dense decoder's 1e-3 with a window that the positions exceed."""
+    from conftest import assert_close_rel
+    from oracle.decode import decode_step
+
+    from machinelearning_b200.paged_decode import PagedGemma3Decoder
+    cfg = small_config()
+    w = host_weights(oracle, cfg, seed=74)
+    for window in (1, 3, 15):
+        model = PagedGemma3Decoder(cfg, w, batch=2, cache_dtype=torch.float32, window=window)
+        model.start(0)
+        if use_graph:
+            model.capture()
+        shape = (1, cfg.n_kv_heads, cfg.ctx, cfg.head_dim)
+        caches = [[[np.zeros(shape, np.float32) for _ in range(cfg.n_layers)] for _ in range(2)] for _ in range(2)]
+        tokens = np.random.default_rng(window).integers(0, cfg.vocab, (2, cfg.ctx))
+        for step in range(cfg.ctx):
+            if step == 2:
+                model.start(1)
+            model.step([tokens[0, step], tokens[1, max(0, step - 2)]])
+            got = model.logits.cpu().numpy()
+            for s in range(2 if step >= 2 else 1):
+                at = step - 2 * s
+                ref = decode_step(cfg, w, tokens[s, at:at + 1], at, *caches[s], window=window)[0]
+                assert_close_rel(got[s], ref, 1e-3, 1e-2)
+        model.close()
+
+
+def test_slots_after_every_eviction(oracle, torch):
+    from machinelearning_b200.paged_decode import PagedGemma3Decoder
+    cfg = small_config()
+    model = PagedGemma3Decoder(cfg, host_weights(oracle, cfg, seed=75), batch=2, budget=4, recent=2)
+    model.start(0)
+    counts = [0, -1]
+    for step in range(12):
+        if step == 3:
+            model.start(1)
+            counts[1] = 0
+        model.step([step, 20 + step])
+        counts = [c + 1 if c >= 0 else c for c in counts]
+        if step % 3 == 2:
+            model.evict()
+            counts = [min(c, 4) for c in counts]
+        assert model.slots.tolist() == [max(c, 0) for c in counts]
+        for li in model.global_layers:  # every held slot has a position of its own, the newest among them
+            for s, c in enumerate(counts):
+                held = model.slot_positions[li][s, 0, :max(c, 0)].tolist()
+                assert len(set(held)) == len(held) and (c <= 0 or max(held) == model.host_positions[s] - 1)
+    model.close()
