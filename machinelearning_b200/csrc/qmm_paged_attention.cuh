@@ -557,10 +557,15 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
             issue(i + 1, pages, a.kv.k, spare, false);
             const Pages after = pages_of(i + 2);
             const uint8_t* src = k_src + at * S::kUnit;
-            static_assert(S::kChunks % 2 == 0, "runs divide a row");
-            // scores: per 8 slots and set two chains of products, of four units of the row at most (the
-            // instruction cuts off where it adds; longer chains were what f32 caches lost most by)
-            constexpr int kX = kSlots / 4, kR = kSlots / 8 < 2 ? 1 : 2, kRun = S::kChunks % 4 == 0 ? 4 : S::kChunks % 3 == 0 ? 3 : 2;
+            // scores: per 8 slots and set two chains of at most four instructions, whose sums are added in 32
+            // bits (an instruction cuts off where it adds; a unit of f32 or bf16 rows takes two of a chain, one
+            // of f16 rows one). Chains of eight: f32 1.6 times as far from the exact outputs as elementary f32
+            // operations, bf16 1.3 times; of four: 1.3 and 1.1 times, in up to 3% more time (16 heads on one of
+            // 256, bf16: 60 us for 58).
+            constexpr int kX = kSlots / 4, kR = kSlots / 8 < 2 ? 1 : 2;
+            constexpr int kMost = S::kChunks % 4 == 0 ? 4 : (S::kChunks % 3 == 0 ? 3 : 2);  // units of an f16 chain
+            constexpr int kRun = std::is_same_v<T, __half> ? kMost : 2;
+            static_assert(S::kChunks % kRun == 0, "runs divide a row");
             float x[SETS][kX] = {};
 #pragma unroll
             for (int r0 = 0; r0 < kSlots / 8; r0 += kR) {
