@@ -156,11 +156,13 @@ struct Slots {
     int first, n;
     int tile0, tiles;
 };
-template <int kSlots>
+// kWaited: the kernel has waited for the ones before; join_kernel reads lengths before
+// its wait, and from L2.
+template <int kSlots, bool kWaited = false>
 __device__ __forceinline__ Slots slots_of(const AttendArgs& a, int b) {
     Slots s;
     const int64_t cap = a.kv.capacity();
-    const int len = __ldcg(a.lengths + b);  // from L2: join_kernel reads it before its wait
+    const int len = kWaited ? a.lengths[b] : __ldcg(a.lengths + b);
     s.n = len < 0 ? 0 : (len > cap ? (int)cap : len);
     s.first = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
     s.tile0 = s.first / kSlots;
@@ -215,6 +217,7 @@ template <typename S>
 __device__ __forceinline__ Place place_of(const AttendArgs& a, const Scratch& sc, int b) {
     const int heads = a.kv.nkv * sc.head_tiles;
     int64_t total = 0, before = 0;
+#pragma unroll 4
     for (int i = threadIdx.x & 31; i < a.kv.n_seqs; i += 32) {
         const int64_t u = units_of<S>(slots_of<S::kSlots>(a, i), heads);
         total += u;
@@ -253,41 +256,72 @@ struct Shape {
     static_assert(kHeads * kAccRow * 4 <= kUnits * kUnit, "a warp's result fits in its ring");
 };
 
-// The (sequence, head tile) that unit share * nth + shift of the list belongs to;
-// b < 0: none. Every warp adds up the sequences' units by itself, a lane a run of
-// them.
+// The (sequence, head tile) that unit share * nth + shift of the list belongs to, by a
+// warp; b < 0: none. Neighbouring lanes read neighbouring lengths, and join_kernel
+// lets one warp do it: with a run of sequences per lane and every warp reading all of
+// them from L2, 560 sequences of 300 slots, 4/1 heads of 256, took 146 us, 90 of them
+// in join_kernel.
 struct Found {
     int64_t share, base;  // base: the unit of the first step of (b, h)
     int b, h;
     Slots s;
 };
-template <typename S>
+template <typename S, bool kWaited>
 __device__ __forceinline__ Found find(const AttendArgs& a, const Scratch& sc, int64_t nth, int shift) {
-    const int lane = threadIdx.x & 31, heads = a.kv.nkv * sc.head_tiles;
-    const int B = a.kv.n_seqs, per = (B + 31) / 32;
-    int64_t mine = 0;
-    for (int b = lane * per; b < min(B, (lane + 1) * per); ++b) mine += units_of<S>(slots_of<S::kSlots>(a, b), heads);
-    int64_t before = mine;
+    const int lane = threadIdx.x & 31, heads = a.kv.nkv * sc.head_tiles, B = a.kv.n_seqs;
+    auto units_at = [&](int b) {
+        return b < B ? units_of<S>(slots_of<S::kSlots, kWaited>(a, b), heads) : (int64_t)0;
+    };
+    auto scan = [&](int64_t u) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += u;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, u, o);
+            if (lane >= o) u += v;
+        }
+        return u;
+    };
+    int64_t upto = scan(units_at(lane));  // of the first 32 sequences
+    const int64_t first = __shfl_sync(0xffffffffu, upto, 31);
+    int64_t total = first;
+    if (B > 32) {
+        int64_t mine = 0;
+#pragma unroll 4
+        for (int b = 32 + lane; b < B; b += 32) mine += units_at(b);
+        total += warp_sum64(mine);
     }
-    const int64_t total = __shfl_sync(0xffffffffu, before, 31);
-    before -= mine;
     Found f;
     f.share = share_of<S>(total, sc.grid);
     f.b = -1;
     const int64_t unit = f.share * nth + shift;
     if (unit >= total) return f;
-    const int owner = __ffs(__ballot_sync(0xffffffffu, unit >= before && unit < before + mine)) - 1;
-    f.b = owner * per;
-    int64_t off = unit - __shfl_sync(0xffffffffu, before, owner);
-    f.s = slots_of<S::kSlots>(a, f.b);
-    while (off >= units_of<S>(f.s, heads)) {
-        off -= units_of<S>(f.s, heads);
-        f.s = slots_of<S::kSlots>(a, ++f.b);
+    int64_t off = unit;
+    int b0 = 0;  // the 32 sequences that hold it
+    if (off >= first) {
+        off -= first;
+        int64_t held = -1;
+        for (b0 = 32; held < 0;) {
+            int64_t u[4], sum[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) u[r] = units_at(b0 + 32 * r + lane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[r] = warp_sum64(u[r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (held < 0) {
+                    if (off < sum[r]) {
+                        held = u[r];
+                    } else {
+                        off -= sum[r];
+                        b0 += 32;
+                    }
+                }
+        }
+        upto = scan(held);
     }
+    const int owner = __ffs(__ballot_sync(0xffffffffu, off < upto)) - 1;
+    f.b = b0 + owner;
+    if (owner) off -= __shfl_sync(0xffffffffu, upto, owner - 1);
+    f.s = slots_of<S::kSlots, kWaited>(a, f.b);
     f.h = (int)(off / (f.s.tiles + S::kSetup));
     f.base = unit - (off - (int64_t)f.h * (f.s.tiles + S::kSetup)) + S::kSetup;
     return f;
@@ -434,7 +468,7 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
     pdl_wait();
     pdl_launch_dependents();
 
-    const Found found = find<S>(a, sc, blockIdx.x, 0);
+    const Found found = find<S, true>(a, sc, blockIdx.x, 0);
     if (found.b < 0) return;
     const int64_t share = found.share, begin = share * blockIdx.x, end = begin + share;
     int b = found.b, h = found.h;
@@ -860,7 +894,7 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
             h = 0;
             do {
                 if (++b == a.kv.n_seqs) return;
-                s = slots_of<kSlots>(a, b);
+                s = slots_of<kSlots, true>(a, b);
             } while (s.tiles == 0);
         }
         __syncthreads();  // the rings and Q are rewritten
@@ -898,7 +932,13 @@ __device__ __forceinline__ void add_weights(const AttendArgs& a, const Scratch& 
     const int64_t row = block / blocks;
     const int b = (int)(row / a.kv.nkv), kvh = (int)(row - (int64_t)b * a.kv.nkv);
     const int64_t t = ((block - row * blocks) * kThreads + threadIdx.x) * 4;
-    const Place place = place_of<S>(a, sc, b);
+    __shared__ Place place_s;
+    if (threadIdx.x < 32) {
+        const Place p = place_of<S>(a, sc, b);
+        if (threadIdx.x == 0) place_s = p;
+    }
+    __syncthreads();
+    const Place place = place_s;
     const Slots s = slots_of<S::kSlots>(a, b);
     const int64_t at = row * cap + t;
     const bool mine = t < cap && t < s.n && t + 4 > s.first;
@@ -976,22 +1016,30 @@ __global__ void __launch_bounds__(JoinShape<HD, kHeads>::kThreads)
     const int group = a.nq / a.kv.nkv;
     const int unit = threadIdx.x / kCols, col = threadIdx.x - unit * kCols;
     const int grp = unit / kHeads, j = unit - grp * kHeads;
-    Found f;
-    bool divided;
-    if constexpr (kHeads == 1) {
-        const int heads = a.kv.nkv * sc.head_tiles;
-        f.b = blockIdx.x / (unsigned)heads;
-        f.h = blockIdx.x - f.b * (unsigned)heads;
-        const Place place = place_of<S>(a, sc, f.b);
-        f.s = slots_of<S::kSlots>(a, f.b);
-        f.share = place.share;
-        f.base = place.start + (int64_t)f.h * (f.s.tiles + S::kSetup) + S::kSetup;
-        divided = f.s.tiles > 0 && place.pieces<S>(f.h).count > 1;
-    } else {  // that of the last unit of CTA c's share
-        f = find<S>(a, sc, (int64_t)blockIdx.x + 1, -1);
-        const int64_t bound = f.share * (blockIdx.x + 1);
-        divided = f.b >= 0 && f.base < bound && f.base + f.s.tiles > bound && f.base / f.share == blockIdx.x;
+    __shared__ Found found_s;
+    __shared__ bool divided_s;
+    if (threadIdx.x < 32) {
+        Found f;
+        bool divided;
+        if constexpr (kHeads == 1) {
+            const int heads = a.kv.nkv * sc.head_tiles;
+            f.b = blockIdx.x / (unsigned)heads;
+            f.h = blockIdx.x - f.b * (unsigned)heads;
+            const Place place = place_of<S>(a, sc, f.b);
+            f.s = slots_of<S::kSlots>(a, f.b);
+            f.share = place.share;
+            f.base = place.start + (int64_t)f.h * (f.s.tiles + S::kSetup) + S::kSetup;
+            divided = f.s.tiles > 0 && place.pieces<S>(f.h).count > 1;
+        } else {  // that of the last unit of CTA c's share
+            f = find<S, false>(a, sc, (int64_t)blockIdx.x + 1, -1);
+            const int64_t bound = f.share * (blockIdx.x + 1);
+            divided = f.b >= 0 && f.base < bound && f.base + f.s.tiles > bound && f.base / f.share == blockIdx.x;
+        }
+        if (threadIdx.x == 0) found_s = f, divided_s = divided;
     }
+    __syncthreads();
+    const Found f = found_s;
+    const bool divided = divided_s;
     pdl_wait();
     for (int b = blockIdx.x; b < a.kv.n_seqs; b += join_blocks)
         if (blockIdx.y == 0 && slots_of<S::kSlots>(a, b).tiles == 0) {

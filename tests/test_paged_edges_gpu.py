@@ -65,3 +65,33 @@ def test_reserve_refuses_what_attend_would(torch):
             cache.reserve(heads)
     with pytest.raises(ValueError):
         cache.reserve(4, budget=-1)
+
+
+@pytest.mark.parametrize("n_seqs", [1, 2, 31, 32, 33, 64, 159, 160, 161, 288, 289, 1025])
+@pytest.mark.parametrize("kind", ["short", "one long", "last alone", "empty"])
+def test_any_number_of_sequences(torch, n_seqs, kind):
+    """The division of the work over many sequences, most of them empty or short, one or two
+    divided among CTAs; with and without weights."""
+    import numpy as np
+
+    from test_paged_gpu import SPLIT, attend_ref, check, make_cache
+    rng = np.random.default_rng(n_seqs)
+    longest = 600 if n_seqs > 64 else 3000
+    lengths = rng.integers(0, 40, n_seqs)
+    if kind == "one long":
+        lengths[n_seqs // 2] = longest
+    if kind == "last alone":
+        lengths[:] = 0
+        lengths[-1] = longest
+    if kind == "empty":
+        lengths[:] = 0
+    lengths = lengths.tolist()
+    cache = make_cache(torch, n_seqs, longest, 1, 64, "f16", 16, seed=n_seqs)
+    q = torch.randn(n_seqs, 3, 64, device="cuda")
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    w = torch.zeros(n_seqs, 1, cache.capacity, device="cuda")
+    ref, tol, wr, wtol = attend_ref(cache, q, lengths, 0.125, 0, SPLIT["f16"])
+    out = cache.attend(q, n, 0.125)
+    check(out, ref, tol)
+    assert torch.equal(cache.attend(q, n, 0.125, weights=w), out)
+    check(w, wr, wtol)
