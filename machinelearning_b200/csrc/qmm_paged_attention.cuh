@@ -245,7 +245,10 @@ struct Shape {
     static constexpr int kVRows = kTile / 4;                     // V rows of a tile per lane
     static constexpr int kUnit = kSlots * HD * (int)sizeof(T);
     static constexpr int kUnits = 3;
-    static constexpr int kWarps = HD <= 64 || (HD <= 128 && SETS == 1) ? 8 : (HD == 192 && SETS == 1 ? 5 : 4);
+    // Eight warps where their rings leave room for two CTAs on an SM and 128 registers hold the results, else
+    // four (head_dim 192, one set: five 68 us, four 65 us for 16 x 16000 slots, 12/2 heads, bf16, 76 and 67 us
+    // for 8 in f32; head_dim 64, two sets: eight spill, 83 us, four 70 us for 32 x 8000, 64/4 heads, bf16).
+    static constexpr int kWarps = HD <= 128 && SETS == 1 ? 8 : 4;
     static constexpr int kQPairs = kChunks * 2 * 32 * 16;        // of a set: first two parts; a third takes half
     static constexpr int kQBytes = kQPairs + (kParts<T> - 2) * kQPairs / 2;
     static constexpr int kSetup = 163840 / (2 * kUnit);          // a piece's fixed cost in steps: 6 us measured
