@@ -247,8 +247,13 @@ struct Shape {
     static constexpr int kUnits = 3;
     // Eight warps where their rings leave room for two CTAs on an SM and 128 registers hold the results, else
     // four (head_dim 192, one set: five 68 us, four 65 us for 16 x 16000 slots, 12/2 heads, bf16, 76 and 67 us
-    // for 8 in f32; head_dim 64, two sets: eight spill, 83 us, four 70 us for 32 x 8000, 64/4 heads, bf16).
+    // for 8 in f32; head_dim 64, two sets: eight spill, 83 us, four 74 us for 32 x 8000, 64/4 heads, bf16).
     static constexpr int kWarps = HD <= 128 && SETS == 1 ? 8 : 4;
+    // A tile's P V summed apart and added in 32 bits, as the instruction cuts off what it adds to large sums.
+    // Head_dim 64 with two sets has the most steps a warp, and single heads there were more than four times as
+    // far from the exact outputs as elementary f32 operations (70 us without). Elsewhere it brings bf16 from 1.1
+    // to 1.0 and f32 from 1.3 to 1.2 times, for up to 9% more time (64 ragged sequences, 64/8 heads of 128, f16).
+    static constexpr bool kFresh = SETS == 2 && HD == 64;
     static constexpr int kQPairs = kChunks * 2 * 32 * 16;        // of a set: first two parts; a third takes half
     static constexpr int kQBytes = kQPairs + (kParts<T> - 2) * kQPairs / 2;
     static constexpr int kSetup = 163840 / (2 * kUnit);          // a piece's fixed cost in steps: 6 us measured
@@ -764,9 +769,15 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                                                         __float_as_uint(f[2][1]), __float_as_uint(f[3][1]));
 #pragma unroll
                             for (int q = 0; q < SETS; ++q) {
-                                mma<T>(acc[q][j * 2 + e], vl, p[q][u][0].x, p[q][u][0].y);
-                                mma<T>(acc[q][j * 2 + e], vh, p[q][u][1].x, p[q][u][1].y);
-                                mma<T>(acc[q][j * 2 + e], vh, p[q][u][0].x, p[q][u][0].y);
+                                float c[4];
+                                float(&d)[4] = S::kFresh ? c : acc[q][j * 2 + e];
+                                if (S::kFresh) c[0] = c[1] = c[2] = c[3] = 0.0f;
+                                mma<T>(d, vl, p[q][u][0].x, p[q][u][0].y);
+                                mma<T>(d, vh, p[q][u][1].x, p[q][u][1].y);
+                                mma<T>(d, vh, p[q][u][0].x, p[q][u][0].y);
+                                if (S::kFresh)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) acc[q][j * 2 + e][i] += c[i];
                             }
                         }
                     } else {
@@ -779,10 +790,16 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
                                                         __byte_perm(v2[e], v3[e], 0x5410),
                                                         __byte_perm(v2[e], v3[e], 0x7632));
 #pragma unroll
-                            for (int q = 0; q < SETS; ++q)
+                            for (int q = 0; q < SETS; ++q) {
+                                float c[4];
+                                float(&d)[4] = S::kFresh ? c : acc[q][j * 4 + e];
+                                if (S::kFresh) c[0] = c[1] = c[2] = c[3] = 0.0f;
 #pragma unroll
-                                for (int f = kParts<T> - 1; f >= 0; --f)
-                                    mma<T>(acc[q][j * 4 + e], vv, p[q][u][f].x, p[q][u][f].y);
+                                for (int f = kParts<T> - 1; f >= 0; --f) mma<T>(d, vv, p[q][u][f].x, p[q][u][f].y);
+                                if (S::kFresh)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) acc[q][j * 4 + e][i] += c[i];
+                            }
                         }
                     }
                 }
