@@ -256,7 +256,10 @@ struct Shape {
     static constexpr bool kFresh = SETS == 2 && HD == 64;
     static constexpr int kQPairs = kChunks * 2 * 32 * 16;        // of a set: first two parts; a third takes half
     static constexpr int kQBytes = kQPairs + (kParts<T> - 2) * kQPairs / 2;
-    static constexpr int kSetup = 163840 / (2 * kUnit);          // a piece's fixed cost in steps: 6 us measured
+    // A piece's fixed cost, in steps: the time of 160 KB of K and V. With 80 KB for it 64 ragged sequences of
+    // up to 8192 slots, 64/8 heads of 128, f16, take 50 us for 40.5 and one of 512 in f32 11.2 for 12.8; with
+    // 240 KB 40 and 14.4.
+    static constexpr int kSetup = 163840 / (2 * kUnit);
     static constexpr int kAccRow = HD + 4;                       // floats; spreads the rows over the banks
     static constexpr size_t kSmem =
         (size_t)kWarps * kUnits * kUnit + SETS * kQBytes + kWarps * kHeads * 8 + kHeads * 4;
@@ -925,9 +928,8 @@ __global__ void __launch_bounds__(Shape<T, HD, SETS>::kWarps * 32, Shape<T, HD, 
 // that left them, and writes the zeros of sequences without slots. Few head tiles
 // with many pieces: a CTA per head (kHeads 1). Many head tiles: a CTA per CTA of
 // attend_kernel, for the one head tile at most that it begins and does not end,
-// eight heads at once (256 sequences of up to 300 slots, 64/8 heads of 128: a CTA
-// per head tile took 4 us longer to find that it had nothing to do). A thread sums
-// four columns of a head over every kGroups-th piece.
+// eight heads at once. A thread sums four columns of a head over every kGroups-th
+// piece.
 // It is on the way of every small call, so it is launched early (programmatic
 // dependent launch, once attend_kernel's own wait is over), finds the pieces from
 // the lengths before it waits for attend_kernel, and has one round of loads after
@@ -1155,8 +1157,11 @@ cudaError_t launch(const AttendArgs& a, Scratch sc, int sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int64_t tiles = (int64_t)a.kv.n_seqs * a.kv.nkv * sc.head_tiles;
     const int heads = a.nq / a.kv.nkv < S::kHeads ? a.nq / a.kv.nkv : S::kHeads;
-    // few head tiles: their heads side by side
-    if (tiles * heads <= 8 * sms) return launch_join<T, HD, SETS, 1>(a, sc, heads, st);
+    // Few heads: side by side, each by a CTA; from about two of those per SM on, the CTAs that find nothing to
+    // join cost more (a CTA per head, one per share boundary: 64 heads in pieces of 131071 slots 91.2, 94.1 us;
+    // 256 with a window of 512 15.4, 15.5; 512 heads of 2000 slots 16.4, 16.4; 768 of 300 17.1, 14.5; 1152 of
+    // 1000 22.2, 19.0; 2048 of 1000 39.0, 31.1).
+    if (tiles * heads <= 2 * sms) return launch_join<T, HD, SETS, 1>(a, sc, heads, st);
     return launch_join<T, HD, SETS, 8>(a, sc, SETS, st);
 }
 
