@@ -227,18 +227,28 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) process_logits_kern
     const int n_bias = n_bias_s;
     for (int k = threadIdx.x; k < n_bias; k += kLogitThreads) {
         const int u = bias_id[k], at = bias_at[k];
-        bool first = true, alone = true;
+        bool first = true;
+        int others = 0;
         for (int m = 0; twice_s && m < n_bias; ++m)
-            if (bias_id[m] == u && m != k) alone = false, first = first && bias_at[m] > at;
+            if (bias_id[m] == u && m != k) ++others, first = first && bias_at[m] > at;
         if (!first || !allowed(u)) continue;
         float f = penalised(W::get(word, u), x[u]) + bias_value[k];
-        for (int last = at; !alone;) {  // the others one by one, in the list's order
-            int next = kMaxBias, from = 0;
-            for (int m = 0; m < n_bias; ++m)
-                if (bias_id[m] == u && bias_at[m] > last && bias_at[m] < next) next = bias_at[m], from = m;
-            if (next == kMaxBias) break;
-            f += bias_value[from];
-            last = next;
+        // the others in the list's order: one by one from the slice's, or, many of them (a list padded with one
+        // id, say), by a scan of the whole list (1024 biases, 1000 of them on one token: 62.7 ms one by one)
+        if (others * n_bias <= a.n_bias) {
+            for (int last = at; others > 0; --others) {
+                int next = kMaxBias, from = 0;
+                for (int m = 0; m < n_bias; ++m)
+                    if (bias_id[m] == u && bias_at[m] > last && bias_at[m] < next) next = bias_at[m], from = m;
+                f += bias_value[from];
+                last = next;
+            }
+        } else {
+            const int* ids = a.bias_ids + (int64_t)row * a.n_bias;
+            const float* values = a.bias_values + (int64_t)row * a.n_bias;
+#pragma unroll 4
+            for (int m = at + 1; m < a.n_bias; ++m)
+                if (ids[m] == v0 + u) f += values[m];
         }
         y[u] = f;
     }

@@ -95,3 +95,26 @@ def test_any_number_of_sequences(torch, n_seqs, kind):
     check(out, ref, tol)
     assert torch.equal(cache.attend(q, n, 0.125, weights=w), out)
     check(w, wr, wtol)
+
+
+@pytest.mark.parametrize("same,n", [(2, 1024), (9, 1024), (700, 1024), (1024, 1024), (3, 3), (40, 64)])
+def test_logits_many_biases_of_one_token(torch, same, n):
+    """A bias list padded with one id, and tokens that come up a few times: the values are added
+    one after the other in the list's order, in 32 bits."""
+    import numpy as np
+
+    from machinelearning_b200.logits import process_logits
+    rng = np.random.default_rng(same)
+    rows, vocab = 3, 40000
+    ids = rng.integers(0, vocab, (rows, n)).astype(np.int32)
+    ids[:, rng.permutation(n)[:same]] = 7
+    ids[1, :2] = 39999
+    vals = rng.normal(0, 5, (rows, n)).astype(np.float32)
+    x = rng.normal(0, 4, (rows, vocab)).astype(np.float32)
+    want = x.copy()
+    for r in range(rows):
+        for t, v in zip(ids[r], vals[r]):
+            want[r, t] = np.float32(want[r, t] + v)
+    cu = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    got = process_logits(cu(x), bias_ids=cu(ids), bias_values=cu(vals))
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
