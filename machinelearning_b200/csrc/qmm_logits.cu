@@ -296,7 +296,8 @@ cudaError_t launch_process_logits(const LogitsArgs& a, cudaStream_t st) {
     const bool vec = (((uintptr_t)a.logits ^ (uintptr_t)a.out) & 15) == 0 && (a.rows == 1 || (a.ld - a.ld_out) % 4 == 0);
     // the longest slices that leave two CTAs for every SM
     int slice = kMaxSlice;
-    while (slice > kMinSlice && (int64_t)a.rows * (a.vocab / slice) < 2 * 148) slice /= 2;
+    const int sms = paged_sm_count();
+    while (slice > kMinSlice && (int64_t)a.rows * (a.vocab / slice) < 2 * sms) slice /= 2;
     if (a.max_tokens < (int)Word<true>::kBiased)
         return vec ? launch<true, true>(a, slice, st) : launch<false, true>(a, slice, st);
     return vec ? launch<true, false>(a, slice, st) : launch<false, false>(a, slice, st);

@@ -42,6 +42,15 @@ struct PagedKv {
     }
 };
 
+// SMs of the current device; a B200's where there is none.
+inline int paged_sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        return 148;
+    return sms;
+}
+
 inline int kv_type_size(int dtype) { return dtype == kKvF32 ? 4 : ((dtype == kKvF16 || dtype == kKvBF16) ? 2 : 0); }
 
 template <typename T>

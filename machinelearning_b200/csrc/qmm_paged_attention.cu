@@ -9,14 +9,6 @@ namespace qmm {
 
 namespace {
 
-int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-        return 148;
-    return sms;
-}
-
 size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Carves the workspace; returns its size.
@@ -44,12 +36,12 @@ size_t carve(const PagedKv& kv, int nq, bool weights, int grid, void* base, Atte
 
 size_t paged_attention_workspace(const PagedKv& kv, int nq, bool weights) {
     AttendScratch sc;
-    return carve(kv, nq, weights, sm_count() * kMaxAttendCtas, nullptr, &sc);
+    return carve(kv, nq, weights, paged_sm_count() * kMaxAttendCtas, nullptr, &sc);
 }
 
 cudaError_t launch_paged_attention(const AttendArgs& a, void* ws, cudaStream_t st) {
     if (a.kv.n_seqs <= 0) return cudaSuccess;
-    const int sms = sm_count();
+    const int sms = paged_sm_count();
     AttendScratch sc;
     carve(a.kv, a.nq, a.weights != nullptr, sms * kMaxAttendCtas, ws, &sc);
     switch (a.kv.dtype) {
