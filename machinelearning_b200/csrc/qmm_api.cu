@@ -1041,7 +1041,7 @@ int guarded(F&& body) {
     try {
         return body();
     } catch (...) {
-        return QMM_ERR_INVALID_DATA;
+        return fail(QMM_ERR_INVALID_DATA, "out of memory");  // short enough to need none
     }
 }
 
