@@ -334,7 +334,9 @@ QMM_API int qmm_add_int_dev(int* p_dev, int value, void* stream);
  * (i + 1) * page_size) of sequence s are on page table_dev[s * table_stride + i],
  * i < max_pages; its capacity is max_pages * page_size (at most 2^30). An
  * entry outside [0, n_pages) names no page: its slots are neither written nor
- * attended to. */
+ * attended to. A page may be on the tables of several sequences (a shared prefix) as
+ * long as its slots are only attended to: append and evict write through the table.
+ * With n_seqs 0 the pointers may be null. */
 typedef struct qmm_paged_kv {
     void* k_dev;
     void* v_dev;
@@ -374,9 +376,14 @@ QMM_API int qmm_paged_append_dev(const qmm_paged_kv* kv, const float* qkv_dev, s
  * zeros. q rows ld_q floats apart (a multiple of 4); float pointers 16-byte aligned.
  * weights_dev and weights_out_dev (both or neither; they may be equal), f32
  * [n_seqs][n_kv_heads][capacity]: out = in, plus at each attended slot the sum
- * over the kv head's query heads of the slot's softmax weight. Workspace: the
- * library's, of the current device and `stream`; reserve
- * qmm_paged_attention_workspace_size bytes before a stream capture.
+ * over the kv head's query heads of the slot's softmax weight. A score of -infinity
+ * (an infinite key) has weight 0, and a sequence with none but those gives zeros; one
+ * of +infinity or NaN makes its head's output NaN; 0 times an infinite v is NaN. Sums
+ * are in 32 bits; queries, weights and f32 caches go through the tensor cores as sums
+ * of parts, 22 bits of f32 and f16 caches, 24 of bf16. Workspace: the library's, of
+ * the current device and `stream`; reserve qmm_paged_attention_workspace_size bytes
+ * before a stream capture. With weights it holds a score for every slot of the table
+ * (n_seqs * n_heads * capacity floats), so size tables by what sequences can hold.
  * (attention.rs:545-600) */
 QMM_API size_t qmm_paged_attention_workspace_size(const qmm_paged_kv* kv, int n_heads, int with_weights);
 QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, size_t ld_q, int n_heads,
@@ -389,7 +396,8 @@ QMM_API int qmm_paged_attention_dev(const qmm_paged_kv* kv, const float* q_dev, 
  * - recent, then those with the largest weights_dev (same shape; NaN ranks as
  * -infinity), ties and a surplus of recent slots by the lowest slot. Kept slots
  * at or above `budget` move, in slot order, into the evicted ones below it (k and
- * v in place); weights_out_dev and positions_out_dev (not the inputs) hold the
+ * v in place, so the pages below a sequence's length are on no other sequence's
+ * table, nor twice on its own: others would see the moved rows); weights_out_dev and positions_out_dev (not the inputs) hold the
  * moved arrays, 0 and -1 beyond the new length; lengths_out_dev [n_seqs] (not
  * lengths_dev) the new lengths. Weights and positions 16-byte aligned; at most
  * 65535 (sequence, kv head) rows. Workspace as above. */
@@ -409,8 +417,8 @@ QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, 
  * mask_rows_dev[i] of mask_dev [n_masks][ceil(vocab / 32)] is clear (a state
  * outside [0, n_masks): no mask; mask_rows_dev null: state i). Null tokens_dev,
  * bias_ids_dev or mask_dev: that step is left out; null prompt_lengths_dev: no
- * prompt; null penalties: 1, 0, 0. Ids outside [0, vocab) are ignored. max_tokens
- * is below 2^30. */
+ * prompt; null penalties: 1, 0, 0. Ids outside [0, vocab) are ignored (bias lists
+ * of uneven length are padded with -1). max_tokens is below 2^30. */
 #define QMM_MAX_BIAS 1024
 QMM_API int qmm_process_logits_dev(const float* logits_dev, size_t ld, size_t rows, size_t vocab,
                                    const int* tokens_dev, size_t ld_tokens, size_t max_tokens,

@@ -42,7 +42,8 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None,
       ``mask_rows[row]`` of ``mask`` (int32 [states][ceil(vocab / 32)]) is clear;
       state -1: no mask; without ``mask_rows`` row i uses state i
 
-    ``out`` may be ``logits``. Ids outside the vocabulary are ignored."""
+    ``out`` may be ``logits``. Ids outside the vocabulary are ignored: pad bias lists
+    with -1."""
     if logits.dim() != 2:
         raise _lib.ShapeMismatch(_lib.ERR_SHAPE_MISMATCH, f"logits: {tuple(logits.shape)} is not [rows][vocab]")
     f32, i32 = torch.float32, torch.int32

@@ -121,8 +121,9 @@ class PagedKVCache:
                out: torch.Tensor | None = None) -> torch.Tensor:
         """q [tokens][n_heads][head_dim] of the fused f32 rows ``qkv`` [tokens][(n_heads
         + 2 n_kv_heads) head_dim]; k and v of token i go to slot ``slots[i]`` of
-        sequence ``seqs[i]`` (default: sequence i). ``positions[i]`` picks the row of
-        the cos/sin tables [ctx][head_dim / 2]. Rows with slot -1 store nothing."""
+        sequence ``seqs[i]`` (default: sequence i), on a page that no other sequence
+        shares. ``positions[i]`` picks the row of the cos/sin tables [ctx][head_dim /
+        2]. Rows with slot -1 store nothing."""
         tokens, hd = qkv.shape[0], self.head_dim
         row = (n_heads + 2 * self.n_kv_heads) * hd
         if qkv.numel() != tokens * row:
@@ -155,7 +156,8 @@ class PagedKVCache:
         shape over each sequence's first ``lengths`` slots (the last ``window`` of
         them, 0: all); a sequence of length 0 gives zeros. ``weights`` f32
         [sequences][kv heads][capacity]: every slot's softmax weight, summed over
-        the kv head's query heads, is added (into ``weights_out`` if given)."""
+        the kv head's query heads, is added (into ``weights_out`` if given). The
+        library's workspace then holds sequences * heads * capacity scores."""
         shape = q.shape
         if len(shape) != 3 or shape[0] != self.n_seqs or shape[2] != self.head_dim:
             raise _mismatch(f"q: {tuple(shape)} is not [{self.n_seqs}][heads][{self.head_dim}]")
@@ -183,7 +185,9 @@ class PagedKVCache:
         before ``next_positions``, then those with the largest ``weights``, ties by
         the lowest slot. Kept slots at or above ``budget`` move (k and v in place)
         into the evicted ones below it, in slot order. ``weights`` f32 and
-        ``positions`` int32 [sequences][kv heads][capacity] are not changed."""
+        ``positions`` int32 [sequences][kv heads][capacity] are not changed. A page
+        below a sequence's length may be on no other sequence's row of the table (a
+        shared prefix): rows would move under the other one."""
         i32, f32, check, slots = torch.int32, torch.float32, self._check, self._slots_shape
         args = (check(lengths, "lengths", i32, self._seqs_shape), check(weights, "weights", f32, slots),
                 check(positions, "positions", i32, slots),
