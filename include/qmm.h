@@ -336,7 +336,8 @@ QMM_API int qmm_add_int_dev(int* p_dev, int value, void* stream);
  * entry outside [0, n_pages) names no page: its slots are neither written nor
  * attended to. A page may be on the tables of several sequences (a shared prefix) as
  * long as its slots are only attended to: append and evict write through the table.
- * With n_seqs 0 the pointers may be null. */
+ * With n_seqs 0 the pointers may be null. At most 65535 sequences, kv heads and
+ * query heads. */
 typedef struct qmm_paged_kv {
     void* k_dev;
     void* v_dev;
@@ -418,7 +419,8 @@ QMM_API int qmm_paged_evict_dev(const qmm_paged_kv* kv, const int* lengths_dev, 
  * outside [0, n_masks): no mask; mask_rows_dev null: state i). Null tokens_dev,
  * bias_ids_dev or mask_dev: that step is left out; null prompt_lengths_dev: no
  * prompt; null penalties: 1, 0, 0. Ids outside [0, vocab) are ignored (bias lists
- * of uneven length are padded with -1). max_tokens is below 2^30. */
+ * of uneven length are padded with -1). At most 65535 rows; max_tokens is below
+ * 2^30, vocab below 2^31 - 65536. */
 #define QMM_MAX_BIAS 1024
 QMM_API int qmm_process_logits_dev(const float* logits_dev, size_t ld, size_t rows, size_t vocab,
                                    const int* tokens_dev, size_t ld_tokens, size_t max_tokens,

@@ -68,11 +68,14 @@ class PagedGemma3Decoder(Gemma3Decoder):
         self.caches[0].reserve(cfg.n_heads, weights=bool(self.budget), budget=self.budget, stream=self.stream)
 
     # ---- sequences ---------------------------------------------------------------------
+    def _check_seq(self, seq: int) -> None:
+        if not 0 <= seq < self.batch:
+            raise ValueError(f"sequence {seq} of {self.batch}")
+
     def start(self, seq: int, prompt_length: int = 0) -> None:
         """Begins a sequence at position 0 with an empty cache; the first ``prompt_length``
         tokens count for the repetition penalty only."""
-        if not 0 <= seq < self.batch:
-            raise ValueError(f"sequence {seq} of {self.batch}")
+        self._check_seq(seq)
         with self._ordered():
             self.positions[seq], self.active[seq], self.slots[seq] = 0, 1, 0
             self.prompt_lengths[seq] = prompt_length
@@ -82,6 +85,7 @@ class PagedGemma3Decoder(Gemma3Decoder):
 
     def stop(self, seq: int) -> None:
         """Leaves a sequence idle: its rows of a step store nothing and attend to nothing."""
+        self._check_seq(seq)
         with self._ordered():
             self.positions[seq], self.active[seq], self.slots[seq] = -1, 0, 0
         self.host_positions[seq] = -1

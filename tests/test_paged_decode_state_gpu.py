@@ -157,3 +157,19 @@ def test_slots_after_every_eviction(oracle, torch):
                 held = model.slot_positions[li][s, 0, :max(c, 0)].tolist()
                 assert len(set(held)) == len(held) and (c <= 0 or max(held) == model.host_positions[s] - 1)
     model.close()
+
+
+def test_sequences_that_do_not_exist(oracle, torch):
+    from machinelearning_b200.paged_decode import PagedGemma3Decoder
+    cfg = small_config()
+    model = PagedGemma3Decoder(cfg, host_weights(oracle, cfg, seed=77), batch=2)
+    model.start(0), model.start(1)
+    for seq in (-1, 2):
+        with pytest.raises(ValueError):
+            model.start(seq)
+        with pytest.raises(ValueError):  # -1 named the last one
+            model.stop(seq)
+    assert model.host_positions == [0, 0] and model.positions.tolist() == [0, 0]
+    model.stop(1)
+    assert model.host_positions == [0, -1] and model.positions.tolist() == [0, -1]
+    model.close()
